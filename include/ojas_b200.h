@@ -268,6 +268,105 @@ OJAS_B200_API int ojas_b200_weight_cache_entry(const ojas_b200_weight_cache *cac
 OJAS_B200_API int ojas_b200_embed_rows(ojas_b200_ctx *ctx, uint32_t ggml_type, const void *table, size_t rows, const uint32_t *ids, size_t M,
                                        size_t d, float *x);
 
+/* ---- between a layer's projections: rotary positions, a paged key / value cache, attention over it.  Element types are
+ * named by their GGUF codes; rows are [token][head][dim] with the heads of a token contiguous and a stride in elements
+ * between tokens (0 = contiguous), so the three parts of a fused QKV row are three pointers into it with one stride.
+ * Launches are stream-ordered and capture-safe; nothing here allocates but the two create calls.
+ *
+ * Every *_check function is the argument check of the call of that name, on the host and without a device: 0, or the
+ * status the call would return, with the message in err (may be null). */
+enum { OJAS_B200_F32 = 0, OJAS_B200_F16 = 1, OJAS_B200_BF16 = 30 };
+enum { OJAS_B200_ROPE_HALF = 0, OJAS_B200_ROPE_INTERLEAVED = 1 };
+
+/* Rotation of pair i by pos * f_i radians, f_i = base^(-2i / rot_dim) / freq_factors[i] (host array, may be null), and for
+ * contexts longer than the trained one (scaling may be null):
+ *   orig_len == 0: every f_i is divided by factor;
+ *   orig_len  > 0: by parts.  A pair that turns r_i = orig_len * f_i / 2 pi times within the original context keeps its
+ *                  frequency for r_i >= beta_fast, has it divided by factor for r_i <= beta_slow, and is mixed linearly in
+ *                  r_i between.
+ * Rotated values are multiplied by magnitude.  create allocates rot_dim / 2 words on the device and copies them there (it
+ * waits for the copy: set-up only); destroy frees them, after the launches that use them have ended. */
+typedef struct ojas_b200_rope ojas_b200_rope;
+typedef struct {
+    double factor, beta_fast, beta_slow;
+    size_t orig_len;
+    float magnitude;
+} ojas_b200_rope_scaling;
+OJAS_B200_API int ojas_b200_rope_create(ojas_b200_ctx *ctx, size_t rot_dim, double base, const ojas_b200_rope_scaling *scaling,
+                                        const float *freq_factors, ojas_b200_rope **out);
+OJAS_B200_API void ojas_b200_rope_destroy(ojas_b200_rope *rope);
+/* The frequencies f_i alone (host): rot_dim / 2 values in radians per position. */
+OJAS_B200_API int ojas_b200_rope_frequencies(size_t rot_dim, double base, const ojas_b200_rope_scaling *scaling, const float *freq_factors,
+                                             double *radians_out, char *err, size_t errlen);
+/* y[m, h, :] = x[m, h, :] with the first rot_dim elements turned by position pos[m] (device, any int32, negative ones turn
+ * back).  layout: pairs are (i, i + rot_dim / 2) (half) or (2i, 2i + 1) (interleaved).  dim even, at most 2048.  Angles are exact
+ * to 2e-9 radians at every position.  x and y may be the same rows (same type and stride); otherwise they must not overlap. */
+OJAS_B200_API int ojas_b200_rope_rows(ojas_b200_ctx *ctx, const ojas_b200_rope *rope, int layout, uint32_t x_type, const void *x, size_t x_stride,
+                                      uint32_t y_type, void *y, size_t y_stride, const int32_t *pos, size_t M, size_t heads, size_t dim);
+OJAS_B200_API int ojas_b200_rope_rows_check(size_t rot_dim, int layout, uint32_t x_type, const void *x, size_t x_stride, uint32_t y_type,
+                                            const void *y, size_t y_stride, const int32_t *pos, size_t M, size_t heads, size_t dim, char *err,
+                                            size_t errlen);
+
+/* The cache: caller-owned device memory for `pages` pages of page_size tokens (a multiple of 16) of `heads` heads of dim
+ * (64, 128, 256) values, f16 or bf16; value d of token t of head h of page p is element
+ * p * page_stride + h * head_stride + t * token_stride + d.  Strides are multiples of 8 elements in any order; k and v start
+ * on 16 bytes and share the strides.  One contiguous cache is one page per sequence.  The handle only describes the memory
+ * (create allocates nothing on the device) and may be used by any context of the same device; destroy leaves the memory alone. */
+typedef struct ojas_b200_kv ojas_b200_kv;
+OJAS_B200_API int ojas_b200_kv_create(ojas_b200_ctx *ctx, uint32_t type, void *k, void *v, size_t pages, size_t page_size, size_t heads, size_t dim,
+                                      size_t page_stride, size_t head_stride, size_t token_stride, ojas_b200_kv **out);
+OJAS_B200_API int ojas_b200_kv_check(uint32_t type, const void *k, const void *v, size_t pages, size_t page_size, size_t heads, size_t dim,
+                                     size_t page_stride, size_t head_stride, size_t token_stride, char *err, size_t errlen);
+OJAS_B200_API void ojas_b200_kv_destroy(ojas_b200_kv *kv);
+
+/* A batch of sequences, all arrays on the device and read by the kernels (a replayed graph sees their current values).
+ * Sequence b owns rows cu[b] .. cu[b + 1] - 1 of the call as its newest tokens and is len[b] tokens long WITH them; its token at
+ * position p is in page table[b * table_stride + p / page_size].  A sequence may have no new row.  Rows outside
+ * cu[0] .. cu[n_seqs] belong to no sequence and are neither read for a result nor written.  max_rows and max_len are host
+ * bounds on the new rows and the length of any sequence: kernels are chosen and split by them.  Entries of the table are
+ * read only for tokens that are needed (under a window, entries in front of it may be anything).
+ * A description that leads outside the cache or the call touches no memory there: such a token is not appended, such a key
+ * reads as zeros, rows beyond max_rows may be left out, and ojas_b200_sync returns OJAS_B200_E_DEVICE. */
+typedef struct {
+    const int32_t *cu;          /* [n_seqs + 1] */
+    const int32_t *len;         /* [n_seqs] */
+    const int32_t *table;       /* [n_seqs][table_stride] */
+    size_t n_seqs, table_stride, max_rows, max_len;
+} ojas_b200_seqs;
+/* The same conditions checked on host copies of the arrays. */
+OJAS_B200_API int ojas_b200_seqs_check_host(const int32_t *cu, const int32_t *len, const int32_t *table, size_t n_seqs, size_t table_stride,
+                                            size_t max_rows, size_t max_len, size_t pages, size_t page_size, size_t M, char *err, size_t errlen);
+/* Stores k and v of the call's M rows at their sequences' newest positions, k rotated (rope null: as it is), both rounded to
+ * the cache's type (beyond f16's range: infinite), and writes q rotated to q_out (q_heads = 0: no q).  A row is turned by its position in its sequence, or by
+ * pos[row] where pos is given.  x_type is the type of q, k and v.  Two sequences whose newest tokens share a page slot would
+ * write the same row: give such tokens pages of their own. */
+OJAS_B200_API int ojas_b200_kv_append(ojas_b200_ctx *ctx, const ojas_b200_kv *kv, const ojas_b200_seqs *seqs, const ojas_b200_rope *rope, int layout,
+                                      uint32_t x_type, const void *q, size_t q_stride, const void *k, size_t k_stride, const void *v,
+                                      size_t v_stride, uint32_t q_type, void *q_out, size_t q_out_stride, size_t q_heads, const int32_t *pos,
+                                      size_t M);
+OJAS_B200_API int ojas_b200_kv_append_check(size_t kv_heads, size_t dim, size_t rot_dim, int layout, uint32_t x_type, const void *q, size_t q_stride,
+                                            const void *k, size_t k_stride, const void *v, size_t v_stride, uint32_t q_type, const void *q_out,
+                                            size_t q_out_stride, size_t q_heads, const int32_t *pos, const ojas_b200_seqs *seqs, size_t M,
+                                            char *err, size_t errlen);
+
+/* out[row, h] = softmax_j(scale * q[row, h] . k_j) v_j over the keys the row sees: of its sequence's first len[b] keys those
+ * up to its own position (causal != 0), or all of them; with window > 0 (causal only) at most the last `window`, its own
+ * included.  q head h reads cache head h / (q_heads / heads).  A row that sees nothing gives zeros.  q and out have type
+ * act_type: f32, or the cache's type; they start on 16 bytes, strides are multiples of 4 elements, and they must not overlap.
+ * f32 activations keep 22 bits through both products over an f16 cache, 16 over a bf16 cache; 16-bit ones are rounded where
+ * the probabilities enter the second product and at the end.  Sums and softmax statistics are f32.
+ * Behind a sequence's end the cache may hold anything; a key that only some rows of a call see must be finite for the
+ * others.  workspace: caller-owned scratch of ojas_b200_attention_workspace_bytes (0: may be null), 256-byte aligned, not
+ * shared by calls that may run at the same time. */
+OJAS_B200_API size_t ojas_b200_attention_workspace_bytes(ojas_b200_ctx *ctx, const ojas_b200_kv *kv, const ojas_b200_seqs *seqs, size_t M,
+                                                         size_t q_heads, long long window);
+OJAS_B200_API int ojas_b200_attention(ojas_b200_ctx *ctx, const ojas_b200_kv *kv, const ojas_b200_seqs *seqs, uint32_t act_type, const void *q,
+                                      size_t q_stride, size_t q_heads, float scale, int causal, long long window, void *out, size_t out_stride,
+                                      size_t M, void *workspace, size_t workspace_bytes);
+OJAS_B200_API int ojas_b200_attention_check(uint32_t cache_type, size_t page_size, size_t kv_heads, size_t dim, uint32_t act_type, size_t q_heads,
+                                            const void *q, size_t q_stride, const void *out, size_t out_stride, float scale, int causal,
+                                            long long window, const ojas_b200_seqs *seqs, size_t M, char *err, size_t errlen);
+
 /* ---- expert residency: replaces ExpertCache (crates/ojas-cuda/src/expert_cache.rs:34-160).  A bounded arena of
  * expert-sized slots in device memory with least-recently-used eviction; misses are streamed from the host through
  * pinned staging memory and re-laid into tiles on the device.  gather() returns byte offsets into the arena: what the

@@ -1,0 +1,486 @@
+// Attention of new tokens over a paged cache:
+//     out[t, h] = sum_j p_j v_j / sum_j p_j,   p_j = exp(scale q[t, h] . k_j - m),   j over the keys that row (t, h) sees,
+// one pass over the keys with the running maximum m and sum of each row (a row that sees nothing gives 0).  This file holds the
+// kernel for few rows per key head (decoding, checking a few drafted tokens), the joining of split rows, and the entry point;
+// attention_tc.cu the tcgen05 kernel for more rows.
+//
+// Few rows are bound by the bytes of K and V (HBM): rows * 4 flops per key byte are far below what even the warp-level MMA
+// gives.  A CTA takes one tile of 8 MT rows of one key head and a range of keys; a producer warp keeps a ring of 64-key blocks
+// of K and V in flight (tensor copies straight from the pages, 128-byte swizzle), four warps take 16 keys of each block with
+// their own running maximum and sum and are joined at the end.
+//
+// mma.m16n8k16 wants 16 rows and a tile has 8: the other 8 carry the LOW halves.  A row of q is two terms of the cache's type,
+// q = hi + lo, in rows g and g + 8 of the A operand, so one instruction forms hi.k and lo.k and the score is their sum; the
+// probabilities go into the second product the same way.  f32 activations over an f16 cache therefore keep 22 bits through
+// both products at no cost in instructions, over a bf16 cache 16 bits (a bf16 term has 8).  f32 rows are scaled by a power of two first so
+// that neither term can overflow or lose bits to f16's range; probabilities are kept scaled by 2^8 for the same reason.
+#include "attention.cuh"
+
+// ---------------------------------------------------------------------------- few rows: warp-level MMA
+constexpr int AR_WARPS = 4;                                  // consumer warps
+constexpr int AR_THREADS = (AR_WARPS + 1) * 32;
+constexpr int AR_KEYS = 64;                                  // keys of a block
+constexpr int AR_STAT_BYTES = 1024;                          // barriers and per-warp row statistics
+__host__ __device__ constexpr int ar_stage_bytes(int dim) { return 2 * AR_KEYS * dim * 2; }
+// 96 KB of blocks in flight per CTA, two CTAs per SM (dim 256: three 64 KB blocks, one CTA): HBM needs about 44 KB per SM and
+// microsecond of latency.
+__host__ __device__ constexpr int ar_stages(int dim) { return dim == 64 ? 6 : 3; }
+__host__ __device__ constexpr int ar_smem(int dim) { return ar_stages(dim) * ar_stage_bytes(dim) + AR_STAT_BYTES + 1024; }
+constexpr float AR_SHIFT = 8.0f, AR_SLACK = 7.0f;            // p <= 2^(SHIFT + SLACK) < 65504; the maximum may lag by SLACK
+
+template <bool BF>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if (BF)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void ldsm4_trans(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+// Address of element (row, col) of a block in shared memory: slabs of 64 columns, rows of 128 bytes, 16-byte pieces swizzled by the
+// row's low three bits (what the tensor copy writes).
+__device__ __forceinline__ uint32_t block_addr(uint32_t base, int row, int col) {
+    return base + (uint32_t)((col >> 6) * (AR_KEYS * 128) + row * 128 + ((((col & 63) >> 3) ^ (row & 7)) << 4));
+}
+// v = hi + lo with both of the 16-bit type, two values packed.
+template <bool BF>
+__device__ __forceinline__ void split_pair(float a, float b, uint32_t &hi, uint32_t &lo) {
+    hi = pack_half(a, b, BF);
+    const float2 h = unpack_half(hi, BF);
+    lo = pack_half(a - h.x, b - h.y, BF);
+}
+
+template <int D, bool BF, int MT>
+__global__ void __launch_bounds__(AR_THREADS, D == 256 || MT == 2 ? 1 : 2) attn_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                                                              const AttnArgs a, int box_rows) {
+    constexpr int STAGES = ar_stages(D), STAGE = ar_stage_bytes(D), HALF = STAGE / 2, ROWS = 8 * MT, NT = D / 8;
+    extern __shared__ unsigned char ar_raw[];
+    unsigned char *smem = reinterpret_cast<unsigned char *>(((uintptr_t)ar_raw + 1023) & ~(uintptr_t)1023);
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + STAGES * STAGE), *empty = full + STAGES;
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(empty + STAGES);
+    float2 *stats = reinterpret_cast<float2 *>(smem + STAGES * STAGE + 256);      // [AR_WARPS][ROWS] (maximum, sum)
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kvh = blockIdx.y, split = blockIdx.z;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; s++) { mbar_init(&full[s], 1); mbar_init(&empty[s], AR_WARPS); }
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&map_k) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&map_v) : "memory");
+    }
+    grid_launch_dependents();
+    grid_dependency_wait();                                  // q, the cache and the batch come from the kernels before this one
+    __syncthreads();
+    RowTile t;
+    if (!find_tile(a, blockIdx.x, ROWS, lane, t)) return;    // the same answer in every warp
+    const int rows = min(ROWS, t.n_rows - t.row0);
+    int lo, hi;
+    key_range(a, t, t.row0, t.row0 + rows, lo, hi);
+    const int blk_all0 = lo / AR_KEYS, blk_all1 = hi > lo ? (hi + AR_KEYS - 1) / AR_KEYS : blk_all0;
+    // (the last split takes all that is left: the result does not depend on the bounds the split was planned with)
+    const bool alone = a.splits == 1 || blk_all1 - blk_all0 <= a.split_blocks;   // this tile has one split: straight to out
+    if (alone && split > 0) return;
+    const int blk0 = min(blk_all1, blk_all0 + split * a.split_blocks);
+    const int blk1 = split == a.splits - 1 ? blk_all1 : min(blk_all1, blk0 + a.split_blocks);
+
+    if (warp == AR_WARPS) {
+        // ---------------- producer: lane = one box (64 values x box_rows tokens) of K or V
+        const int per_slab = AR_KEYS / box_rows, boxes = 2 * per_slab * (D / 64);
+        uint32_t phase = 1;
+        int s = 0;
+        for (int blk = blk0; blk < blk1; blk++) {
+            if (!mbar_wait_warp(&empty[s], phase, abort_flag, a.batch.status, OJAS_ST_ATTN_WAIT)) break;
+            const int part = lane % per_slab, slab = lane / per_slab % (D / 64), key = blk * AR_KEYS + part * box_rows;
+            const bool is_v = lane >= boxes / 2;
+            const bool want = lane < boxes && key < hi && key + box_rows > lo;
+            int page = 0;
+            if (want) {
+                page = __ldg(a.batch.table + (long long)t.seq * a.batch.table_stride + key / a.batch.page_size);
+                if (page < 0 || page >= a.batch.pages) { atomicOr(a.batch.status, OJAS_ST_BATCH); page = a.batch.pages; }   // reads as zeros
+            }
+            const int n = __popc(__ballot_sync(0xffffffffu, want));
+            if (lane == 0) mbar_arrive_expect_tx(&full[s], (uint32_t)(n * box_rows * 128));
+            __syncwarp();
+            if (want)
+                tma_load_4d(smem + s * STAGE + (is_v ? HALF : 0) + slab * (AR_KEYS * 128) + part * box_rows * 128, is_v ? &map_v : &map_k, slab * 64,
+                            key % a.batch.page_size, kvh, page, &full[s]);
+            if (++s == STAGES) { s = 0; phase ^= 1u; }
+        }
+    }
+    float o[MT][NT][4];
+    float m[MT], l[MT];
+    if (warp < AR_WARPS) {
+        const int g = lane >> 2, q4 = lane & 3;
+#pragma unroll
+        for (int i = 0; i < MT; i++) {
+            m[i] = -INFINITY; l[i] = 0.0f;
+#pragma unroll
+            for (int n = 0; n < NT; n++) o[i][n][0] = o[i][n][1] = o[i][n][2] = o[i][n][3] = 0.0f;
+        }
+        // ---------------- q: this lane's pairs of row g, as hi (rows 0..7 of the MMA tile) and lo (rows 8..15)
+        uint32_t qf[MT][D / 16][4];
+        float factor[MT];                                    // score -> log2 units
+        int see_lo[MT], see_hi[MT];
+#pragma unroll
+        for (int i = 0; i < MT; i++) {
+            const int row = t.row0 + 8 * i + g;
+            const bool live = 8 * i + g < rows;
+            see_lo[i] = see_hi[i] = 0;
+            factor[i] = a.scale_log2;
+            const long long at = live ? (long long)(t.token0 + row / a.group) * a.q_stride + (long long)(kvh * a.group + row % a.group) * D : 0;
+            if (live) row_range(a, t, row, see_lo[i], see_hi[i]);
+            if (a.act_type == OJAS_B200_F32) {
+                const float *q = static_cast<const float *>(a.q) + at;
+                float2 v[D / 8];
+                float top = 0.0f;
+#pragma unroll
+                for (int k = 0; k < D / 8; k++) {
+                    v[k] = live ? make_float2(__ldg(q + k * 8 + 2 * q4), __ldg(q + k * 8 + 2 * q4 + 1)) : make_float2(0.f, 0.f);
+                    top = fmaxf(top, fmaxf(fabsf(v[k].x), fabsf(v[k].y)));
+                }
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                // 2^e in (top/2, top]: the row over 2^e is below 2 (zero, infinite and subnormal rows stay as they are)
+                const uint32_t e = __float_as_uint(top) & 0x7f800000u;
+                const bool scalable = e > 0x01000000u && e < 0x7e000000u;
+                const float up = scalable ? __uint_as_float(e) : 1.0f, down = scalable ? __uint_as_float(0x7f000000u - e) : 1.0f;
+                factor[i] *= up;
+#pragma unroll
+                for (int k = 0; k < D / 16; k++) {
+                    split_pair<BF>(v[2 * k].x * down, v[2 * k].y * down, qf[i][k][0], qf[i][k][1]);
+                    split_pair<BF>(v[2 * k + 1].x * down, v[2 * k + 1].y * down, qf[i][k][2], qf[i][k][3]);
+                }
+            } else {
+                const uint16_t *q = static_cast<const uint16_t *>(a.q) + at;
+#pragma unroll
+                for (int k = 0; k < D / 16; k++) {
+                    qf[i][k][0] = live ? (uint32_t)__ldg(q + k * 16 + 2 * q4) | (uint32_t)__ldg(q + k * 16 + 2 * q4 + 1) << 16 : 0u;
+                    qf[i][k][2] = live ? (uint32_t)__ldg(q + k * 16 + 8 + 2 * q4) | (uint32_t)__ldg(q + k * 16 + 8 + 2 * q4 + 1) << 16 : 0u;
+                    qf[i][k][1] = qf[i][k][3] = 0u;
+                }
+            }
+        }
+        const int mi = lane >> 3, mr = lane & 7;             // ldmatrix: which 8x8 matrix this lane addresses, and its row
+        uint32_t phase = 0;
+        int s = 0;
+        for (int blk = blk0; blk < blk1; blk++) {
+            if (!mbar_wait_warp(&full[s], phase, abort_flag, a.batch.status, OJAS_ST_ATTN_WAIT)) break;
+            const int key0 = blk * AR_KEYS + warp * 16;
+            const uint32_t kb = smem_u32(smem + s * STAGE), vb = kb + HALF;
+            if (key0 < hi && key0 + 16 > lo) {
+                if (key0 < lo || key0 + 16 > hi) {
+                    // what lies behind the sequence or was not copied may be anything, and 0 * NaN is NaN: this warp's keys outside
+                    // [lo, hi) get zeros for values
+                    for (int i = lane; i < 16 * (D / 8); i += 32) {
+                        const int r = i / (D / 8), c = i % (D / 8) * 8;
+                        if (key0 + r < lo || key0 + r >= hi)
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(block_addr(vb, warp * 16 + r, c)), "r"(0) : "memory");
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // before the next copy into this stage
+                    __syncwarp();
+                }
+                float sc[MT][2][4];
+#pragma unroll
+                for (int i = 0; i < MT; i++)
+#pragma unroll
+                    for (int n = 0; n < 2; n++) sc[i][n][0] = sc[i][n][1] = sc[i][n][2] = sc[i][n][3] = 0.0f;
+#pragma unroll
+                for (int k = 0; k < D / 16; k++) {
+                    uint32_t b[4];
+                    ldsm4(b, block_addr(kb, warp * 16 + (mi >> 1) * 8 + mr, k * 16 + (mi & 1) * 8));
+#pragma unroll
+                    for (int i = 0; i < MT; i++) {
+                        mma16816<BF>(sc[i][0], qf[i][k], b[0], b[1]);
+                        mma16816<BF>(sc[i][1], qf[i][k], b[2], b[3]);
+                    }
+                }
+                uint32_t pf[MT][4];
+#pragma unroll
+                for (int i = 0; i < MT; i++) {
+                    float x[4];                              // keys key0 + 2 q4 + {0, 1, 8, 9} of row g
+#pragma unroll
+                    for (int n = 0; n < 2; n++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            const int key = key0 + n * 8 + 2 * q4 + e;
+                            const float v = (sc[i][n][e] + sc[i][n][e + 2]) * factor[i];
+                            x[2 * n + e] = key >= see_lo[i] && key < see_hi[i] ? v : -INFINITY;
+                        }
+                    float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                    const bool grow = top > m[i] + AR_SLACK;   // (-inf + slack = -inf: the first seen key always raises it)
+                    if (__any_sync(0xffffffffu, grow)) {
+                        const float mn = grow ? top : m[i];
+                        const float f = mn == m[i] ? 1.0f : exp2_fast(m[i] - mn);
+                        m[i] = mn;
+                        l[i] *= f;
+#pragma unroll
+                        for (int n = 0; n < NT; n++) { o[i][n][0] *= f; o[i][n][1] *= f; o[i][n][2] *= f; o[i][n][3] *= f; }
+                    }
+                    const float off = m[i] == -INFINITY ? 0.0f : m[i] - AR_SHIFT;
+                    float p[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) { p[e] = exp2_fast(x[e] - off); l[i] += p[e]; }
+                    split_pair<BF>(p[0], p[1], pf[i][0], pf[i][1]);
+                    split_pair<BF>(p[2], p[3], pf[i][2], pf[i][3]);
+                }
+#pragma unroll
+                for (int n2 = 0; n2 < D / 16; n2++) {
+                    uint32_t b[4];
+                    ldsm4_trans(b, block_addr(vb, warp * 16 + (mi & 1) * 8 + mr, n2 * 16 + (mi >> 1) * 8));
+#pragma unroll
+                    for (int i = 0; i < MT; i++) {
+                        mma16816<BF>(o[i][2 * n2], pf[i], b[0], b[1]);
+                        mma16816<BF>(o[i][2 * n2 + 1], pf[i], b[2], b[3]);
+                    }
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty[s]);
+            if (++s == STAGES) { s = 0; phase ^= 1u; }
+        }
+#pragma unroll
+        for (int i = 0; i < MT; i++) {
+            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+            if (q4 == 0) stats[warp * ROWS + 8 * i + g] = make_float2(m[i], l[i]);
+        }
+    }
+    __syncthreads();                                         // the ring is free: every copy that was issued has been waited for
+    if (*abort_flag) {                                       // copies still in flight get a bounded time to land
+        const long long t0 = clock64();
+        while (clock64() - t0 < 2000000LL) { }
+        return;
+    }
+    // ---------------- the four warps' sums, each scaled to the tile's maximum, meet in shared memory
+    float *sums = reinterpret_cast<float *>(smem);           // [AR_WARPS][ROWS][D]
+    if (warp < AR_WARPS) {
+        const int g = lane >> 2, q4 = lane & 3;
+#pragma unroll
+        for (int i = 0; i < MT; i++) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < AR_WARPS; w++) top = fmaxf(top, stats[w * ROWS + 8 * i + g].x);
+            const float f = m[i] == -INFINITY ? 0.0f : m[i] == top ? 1.0f : exp2_fast(m[i] - top);
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+                *reinterpret_cast<float2 *>(sums + (warp * ROWS + 8 * i + g) * D + n * 8 + 2 * q4) =
+                    make_float2((o[i][n][0] + o[i][n][2]) * f, (o[i][n][1] + o[i][n][3]) * f);
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < rows * (D / 4); i += AR_THREADS) {
+        const int r = i / (D / 4), c = i % (D / 4) * 4, row = t.row0 + r;
+        float top = -INFINITY, total = 0.0f;
+#pragma unroll
+        for (int w = 0; w < AR_WARPS; w++) top = fmaxf(top, stats[w * ROWS + r].x);
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < AR_WARPS; w++) {
+            const float2 st = stats[w * ROWS + r];
+            total += st.x == -INFINITY ? 0.0f : st.x == top ? st.y : st.y * exp2_fast(st.x - top);
+            const float4 x = *reinterpret_cast<const float4 *>(sums + (w * ROWS + r) * D + c);
+            v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+        }
+        const long long token = t.token0 + row / a.group;
+        const int head = kvh * a.group + row % a.group;
+        if (alone) {
+            const float inv = total > 0.0f || total != total ? 1.0f / total : 0.0f;
+            store_elem4(a.out, a.act_type, token * a.out_stride + (long long)head * D + c, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+            if (a.part_ml && c == 0) a.part_ml[token * a.q_heads + head] = make_float2(0.0f, -1.0f);
+        } else {
+            const long long slot = ((long long)split * a.batch.M + token) * a.q_heads + head;
+            if (blk1 > blk0) *reinterpret_cast<float4 *>(a.part_o + slot * D + c) = v;
+            if (c == 0) a.part_ml[slot] = make_float2(top, total);
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------- joining the splits
+// One warp per (token, head): the splits' sums, each scaled to the row's maximum, over the total.  Rows that a kernel finished
+// itself, and rows of no sequence, are left alone.
+template <int D>
+__global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a) {
+    grid_launch_dependents();
+    grid_dependency_wait();
+    const int lane = threadIdx.x & 31;
+    const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5), rows = a.batch.M * a.q_heads;
+    if (row >= rows) return;
+    const long long token = row / a.q_heads;
+    if (token < __ldg(a.batch.cu) || token >= __ldg(a.batch.cu + a.batch.n_seqs)) return;
+    const float2 first = a.part_ml[row];
+    if (first.y < 0.0f) return;
+    float top = -INFINITY;
+    for (int s = lane; s < a.splits; s += 32) top = fmaxf(top, a.part_ml[(long long)s * rows + row].x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    constexpr int V = D / 32;                                // values per lane
+    float acc[V], total = 0.0f;
+#pragma unroll
+    for (int i = 0; i < V; i++) acc[i] = 0.0f;
+    for (int s = 0; s < a.splits; s++) {
+        const float2 ml = a.part_ml[(long long)s * rows + row];
+        if (ml.x == -INFINITY) continue;                     // the split saw no key of this row
+        const float f = ml.x == top ? 1.0f : exp2_fast(ml.x - top);
+        total += ml.y * f;
+        const float *o = a.part_o + ((long long)s * rows + row) * D + lane * V;
+#pragma unroll
+        for (int i = 0; i < V; i += 2) {
+            const float2 x = *reinterpret_cast<const float2 *>(o + i);
+            acc[i] += x.x * f;
+            acc[i + 1] += x.y * f;
+        }
+    }
+    const float inv = total > 0.0f || total != total ? 1.0f / total : 0.0f;
+    const long long at = token * a.out_stride + (row - token * a.q_heads) * D + lane * V;
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+        if (a.act_type == OJAS_B200_F32) *reinterpret_cast<float2 *>(static_cast<float *>(a.out) + at + i) = make_float2(acc[i] * inv, acc[i + 1] * inv);
+        else *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(a.out) + at + i) = pack_half(acc[i] * inv, acc[i + 1] * inv, a.act_type == OJAS_B200_BF16);
+    }
+}
+
+// ---------------------------------------------------------------------------- plan
+static int attn_shape_check(uint32_t cache_type, size_t page_size, size_t kv_heads, size_t dim, uint32_t act_type, size_t q_heads, size_t M, size_t max_rows,
+                            size_t max_len, char *err, size_t errlen) {
+    auto no = [&](int code, const char *why) { if (err && errlen) snprintf(err, errlen, "attention: %s", why); return code; };
+    if (dim != 64 && dim != 128 && dim != 256) return no(OJAS_B200_E_UNSUPPORTED, "the head size must be 64, 128 or 256");
+    if (cache_type != OJAS_B200_F16 && cache_type != OJAS_B200_BF16) return no(OJAS_B200_E_ARG, "a cache holds f16 or bf16");
+    if (act_type != OJAS_B200_F32 && act_type != cache_type) return no(OJAS_B200_E_UNSUPPORTED, "activations must be f32 or the cache's type");
+    if (page_size == 0 || page_size % 16) return no(OJAS_B200_E_UNSUPPORTED, "the page size must be a multiple of 16 tokens");
+    if (kv_heads == 0 || kv_heads > 65535 || q_heads == 0 || q_heads > 65536 || q_heads % kv_heads) return no(OJAS_B200_E_ARG, "query heads must be a multiple of the cache's heads");
+    if (M > 0x3fffffffull || max_rows > 0x3fffffffull || max_len > 0x7fffff00ull || M * (q_heads / kv_heads) > 0x3fffffffull)
+        return no(OJAS_B200_E_LIMIT, "too many rows or keys");
+    return 0;
+}
+
+// Which kernel, and how far the keys are split so that few rows still use every SM.
+static AttnPlan attn_plan(int sm_count, size_t n_seqs, size_t M, size_t max_rows, size_t max_len, size_t q_heads, size_t kv_heads, size_t dim, size_t window) {
+    AttnPlan p{};
+    const size_t group = q_heads / kv_heads, bound = (max_rows < M ? max_rows : M) * group;
+    p.tensor = false;
+    p.mt = bound > 8 && dim <= 128 ? 2 : 1;
+    p.rows = 8 * p.mt;
+    p.block = AR_KEYS;
+    const unsigned long long by_seq = (unsigned long long)n_seqs * ((bound + p.rows - 1) / p.rows), by_row = (unsigned long long)M * group / p.rows + n_seqs;
+    p.tiles = (long long)(by_seq < by_row ? by_seq : by_row);
+    size_t span = max_len;                                   // keys a tile can see at most
+    if (window && window + p.rows < span) span = window + p.rows;
+    const size_t blocks = span / p.block + 2;
+    const long long slots = (long long)sm_count * (dim == 256 ? 1 : 2), ctas = p.tiles * (long long)kv_heads;
+    long long want = ctas >= 4 * slots ? 1 : (2 * slots + ctas - 1) / ctas;
+    const long long most = (long long)((blocks + 3) / 4);    // a split of fewer than 4 blocks costs more to start and join than it saves
+    if (want > most) want = most;
+    if (want > 1024) want = 1024;
+    if (want < 1) want = 1;
+    p.split_blocks = (int)((blocks + want - 1) / want);
+    p.splits = (int)((blocks + p.split_blocks - 1) / p.split_blocks);
+    const size_t rows = M * q_heads;
+    p.workspace = p.splits > 1 ? align256((size_t)p.splits * rows * sizeof(float2)) + (size_t)p.splits * rows * dim * sizeof(float) : 0;
+    return p;
+}
+
+extern "C" int ojas_b200_attention_check(uint32_t cache_type, size_t page_size, size_t kv_heads, size_t dim, uint32_t act_type, size_t q_heads, const void *q,
+                                         size_t q_stride, const void *out, size_t out_stride, float scale, int causal, long long window,
+                                         const ojas_b200_seqs *seqs, size_t M, char *err, size_t errlen) {
+    auto no = [&](int code, const char *why) { if (err && errlen) snprintf(err, errlen, "attention: %s", why); return code; };
+    int rc = seqs_check(seqs, M, err, errlen);
+    if (rc) return rc;
+    rc = attn_shape_check(cache_type, page_size, kv_heads, dim, act_type, q_heads, M, seqs->max_rows, seqs->max_len, err, errlen);
+    if (rc) return rc;
+    if (!(scale == scale) || scale - scale != 0.0f) return no(OJAS_B200_E_ARG, "the scale must be finite");
+    if (window < 0 || window > 0x7fffffff) return no(OJAS_B200_E_ARG, "the window must be 0 (none) or a number of keys");
+    if (window && !causal) return no(OJAS_B200_E_UNSUPPORTED, "a window needs causal rows");
+    if ((q_stride && q_stride < q_heads * dim) || (out_stride && out_stride < q_heads * dim)) return no(OJAS_B200_E_ARG, "a row stride is smaller than a row");
+    if (q_stride > (1ull << 40) || out_stride > (1ull << 40)) return no(OJAS_B200_E_LIMIT, "a stride is too large");
+    if (q_stride % 4 || out_stride % 4) return no(OJAS_B200_E_ARG, "strides must be multiples of 4 elements");
+    if (M && seqs->n_seqs) {
+        if (!q || !out) return no(OJAS_B200_E_ARG, "null pointer");
+        if ((uintptr_t)q % 16 || (uintptr_t)out % 16) return no(OJAS_B200_E_ARG, "q and out must start on 16 bytes");
+    }
+    return 0;
+}
+
+extern "C" size_t ojas_b200_attention_workspace_bytes(ojas_b200_ctx *ctx, const ojas_b200_kv *kv, const ojas_b200_seqs *seqs, size_t M, size_t q_heads, long long window) {
+    if (!ctx || !kv || !seqs || window < 0 || M == 0 || seqs->n_seqs == 0) return 0;
+    if (attn_shape_check(kv->type, kv->page_size, kv->heads, kv->dim, kv->type, q_heads, M, seqs->max_rows, seqs->max_len, nullptr, 0)) return 0;
+    return attn_plan(ctx->sm_count, seqs->n_seqs, M, seqs->max_rows, seqs->max_len, q_heads, kv->heads, kv->dim, (size_t)window).workspace;
+}
+
+template <int D, bool BF, int MT>
+static cudaError_t launch_rows(const ojas_b200_ctx *ctx, const ojas_b200_kv *kv, const AttnArgs &a, const AttnPlan &p) {
+    cudaError_t e = cudaFuncSetAttribute(attn_rows_kernel<D, BF, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, ar_smem(D));
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)p.tiles, (unsigned)kv->heads, (unsigned)p.splits);
+    cfg.blockDim = dim3(AR_THREADS);
+    cfg.dynamicSmemBytes = ar_smem(D);
+    cfg.stream = ctx->stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = ctx->pdl ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, attn_rows_kernel<D, BF, MT>, kv->map_k, kv->map_v, a, kv->box_rows);
+}
+template <bool BF>
+static cudaError_t launch_rows_dim(const ojas_b200_ctx *ctx, const ojas_b200_kv *kv, const AttnArgs &a, const AttnPlan &p) {
+    if (kv->dim == 64) return p.mt == 2 ? launch_rows<64, BF, 2>(ctx, kv, a, p) : launch_rows<64, BF, 1>(ctx, kv, a, p);
+    if (kv->dim == 128) return p.mt == 2 ? launch_rows<128, BF, 2>(ctx, kv, a, p) : launch_rows<128, BF, 1>(ctx, kv, a, p);
+    return launch_rows<256, BF, 1>(ctx, kv, a, p);
+}
+
+extern "C" int ojas_b200_attention(ojas_b200_ctx *ctx, const ojas_b200_kv *kv, const ojas_b200_seqs *seqs, uint32_t act_type, const void *q, size_t q_stride,
+                                   size_t q_heads, float scale, int causal, long long window, void *out, size_t out_stride, size_t M, void *workspace,
+                                   size_t workspace_bytes) {
+    if (!ctx) return OJAS_B200_E_ARG;
+    if (!kv) return ojas_fail(ctx, OJAS_B200_E_ARG, "attention: null cache");
+    if (kv->ctx->device != ctx->device) return ojas_fail(ctx, OJAS_B200_E_ARG, "attention: the cache lives on device %d, the context on %d", kv->ctx->device, ctx->device);
+    char why[256];
+    const int rc = ojas_b200_attention_check(kv->type, kv->page_size, kv->heads, kv->dim, act_type, q_heads, q, q_stride, out, out_stride, scale, causal, window, seqs, M, why, sizeof why);
+    if (rc) return ojas_fail(ctx, rc, "%s", why);
+    if (M == 0 || seqs->n_seqs == 0) return 0;
+    const AttnPlan p = attn_plan(ctx->sm_count, seqs->n_seqs, M, seqs->max_rows, seqs->max_len, q_heads, kv->heads, kv->dim, (size_t)window);
+    if (p.workspace) {
+        if (!workspace || workspace_bytes < p.workspace) return ojas_fail(ctx, OJAS_B200_E_ARG, "attention: workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : 0, p.workspace);
+        if ((uintptr_t)workspace % 256) return ojas_fail(ctx, OJAS_B200_E_ARG, "attention: the workspace must start on 256 bytes");
+    }
+    if (p.tiles > 0x7fffffffll || p.splits > 65535) return ojas_fail(ctx, OJAS_B200_E_LIMIT, "attention: too many row tiles");
+    AttnArgs a{};
+    a.q = q; a.out = out;
+    a.q_stride = (long long)(q_stride ? q_stride : q_heads * kv->dim);
+    a.out_stride = (long long)(out_stride ? out_stride : q_heads * kv->dim);
+    a.batch = {seqs->cu, seqs->len, seqs->table, (int)seqs->n_seqs, (int)seqs->table_stride, (long long)M, (int)kv->pages, (int)kv->page_size, (int)seqs->max_rows, ctx->dev_status};
+    a.act_type = act_type; a.q_heads = (int)q_heads; a.group = (int)(q_heads / kv->heads);
+    a.splits = p.splits; a.split_blocks = p.split_blocks;
+    a.window = (int)window; a.causal = causal != 0;
+    a.scale_log2 = scale * 1.4426950408889634f;
+    if (p.workspace) {
+        a.part_ml = static_cast<float2 *>(workspace);
+        a.part_o = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + align256((size_t)p.splits * M * q_heads * sizeof(float2)));
+    }
+    DeviceGuard guard(ctx->device);
+    cudaError_t e = kv->type == OJAS_B200_BF16 ? launch_rows_dim<true>(ctx, kv, a, p) : launch_rows_dim<false>(ctx, kv, a, p);
+    if (e != cudaSuccess) return ojas_fail(ctx, OJAS_B200_E_CUDA, "launch attn_rows: %s", cudaGetErrorString(e));
+    OJAS_LAUNCH_CHECK(ctx, "attn_rows");
+    if (p.splits > 1) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)((M * q_heads + 7) / 8)); cfg.blockDim = dim3(256); cfg.stream = ctx->stream;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = ctx->pdl ? 1 : 0;
+        e = kv->dim == 64 ? cudaLaunchKernelEx(&cfg, attn_join_kernel<64>, a)
+                          : kv->dim == 128 ? cudaLaunchKernelEx(&cfg, attn_join_kernel<128>, a) : cudaLaunchKernelEx(&cfg, attn_join_kernel<256>, a);
+        if (e != cudaSuccess) return ojas_fail(ctx, OJAS_B200_E_CUDA, "launch attn_join: %s", cudaGetErrorString(e));
+        OJAS_LAUNCH_CHECK(ctx, "attn_join");
+    }
+    return 0;
+}

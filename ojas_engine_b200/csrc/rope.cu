@@ -1,0 +1,175 @@
+// Rotary positions: pair i of a head is turned by the angle pos * f_i,
+//     (a, b) -> magnitude * (a cos - b sin, b cos + a sin),
+// f_i = base^(-2i / rot_dim), scaled for contexts longer than the trained one.  Pairs are (x[i], x[i + rot_dim/2]) (half) or
+// (x[2i], x[2i + 1]) (interleaved); elements from rot_dim on pass through.
+//
+// Angles: a 32-bit product pos * f_i is wrong by 0.06 radians at position 10^6.  The frequency is kept in turns as a 64-bit
+// binary fraction instead: pos * turns wraps modulo 2^64, i.e. modulo one turn, without any rounding, and its top bits go to
+// sincospi.  What is left is the rounding of f_i to 2^-64 turns and of the fraction to 32 bits (2^-32 turns = 1.5e-9 rad).
+#include <math.h>
+
+#include "attn.cuh"
+#include "rope.cuh"
+
+// The frequencies in radians per position (host, 64 bits).
+static int rope_frequencies(size_t rot_dim, double base, const ojas_b200_rope_scaling *sc, const float *freq_factors, double *f, char *err, size_t errlen) {
+    auto no = [&](const char *why) { if (err && errlen) snprintf(err, errlen, "rope: %s", why); return OJAS_B200_E_ARG; };
+    if (rot_dim < 2 || rot_dim % 2 != 0 || rot_dim > 1024) return no("rot_dim must be even, 2..1024");
+    if (!(base > 1.0) || !isfinite(base)) return no("base must be a finite number above 1");
+    const double factor = sc ? sc->factor : 1.0, fast = sc ? sc->beta_fast : 0.0, slow = sc ? sc->beta_slow : 0.0;
+    if (!(factor > 0.0) || !isfinite(factor)) return no("factor must be positive");
+    if (sc && !(sc->magnitude > 0.0f && isfinite(sc->magnitude))) return no("magnitude must be positive");
+    if (sc && sc->orig_len && !(fast > slow && slow >= 0.0 && isfinite(fast))) return no("beta_fast must be above beta_slow, both finite and not negative");
+    for (size_t i = 0; i < rot_dim / 2; i++) {
+        f[i] = pow(base, -2.0 * (double)i / (double)rot_dim);
+        if (freq_factors) {
+            if (!(freq_factors[i] > 0.0f) || !isfinite(freq_factors[i])) return no("frequency factors must be positive");
+            f[i] /= (double)freq_factors[i];
+        }
+        if (sc && sc->orig_len) {                 // by parts: pairs that turn often within the original context keep their frequency
+            double keep = ((double)sc->orig_len * f[i] / (2.0 * M_PI) - slow) / (fast - slow);
+            keep = keep < 0.0 ? 0.0 : keep > 1.0 ? 1.0 : keep;
+            f[i] = f[i] * keep + f[i] / factor * (1.0 - keep);
+        } else {
+            f[i] /= factor;
+        }
+    }
+    return 0;
+}
+
+extern "C" int ojas_b200_rope_frequencies(size_t rot_dim, double base, const ojas_b200_rope_scaling *scaling, const float *freq_factors,
+                                          double *radians_out, char *err, size_t errlen) {
+    if (!radians_out) return OJAS_B200_E_ARG;
+    return rope_frequencies(rot_dim, base, scaling, freq_factors, radians_out, err, errlen);
+}
+
+extern "C" int ojas_b200_rope_create(ojas_b200_ctx *ctx, size_t rot_dim, double base, const ojas_b200_rope_scaling *scaling, const float *freq_factors,
+                                     ojas_b200_rope **out) {
+    if (!ctx || !out) return OJAS_B200_E_ARG;
+    *out = nullptr;
+    double f[512];
+    uint64_t turns[512];
+    const int rc = rope_frequencies(rot_dim, base, scaling, freq_factors, f, ctx->err, sizeof ctx->err);
+    if (rc) return rc;
+    for (size_t i = 0; i < rot_dim / 2; i++) {
+        const double t = f[i] / (2.0 * M_PI), frac = t - floor(t);           // below one turn per position in all real uses
+        turns[i] = (uint64_t)ldexp(frac, 64);                                // a double has 53 bits: exact
+    }
+    DeviceGuard guard(ctx->device);
+    uint64_t *dev = nullptr;
+    OJAS_CUDA(ctx, cudaMalloc((void **)&dev, rot_dim / 2 * sizeof(uint64_t)));
+    const cudaError_t e = cudaMemcpy(dev, turns, rot_dim / 2 * sizeof(uint64_t), cudaMemcpyHostToDevice);
+    if (e != cudaSuccess) {
+        cudaFree(dev);
+        return ojas_fail(ctx, OJAS_B200_E_CUDA, "rope_create: %s", cudaGetErrorString(e));
+    }
+    ojas_b200_rope *r = new (std::nothrow) ojas_b200_rope();
+    if (!r) { cudaFree(dev); return ojas_fail(ctx, OJAS_B200_E_LIMIT, "rope_create: out of host memory"); }
+    r->ctx = ctx; r->rot_dim = (uint32_t)rot_dim; r->turns = dev;
+    r->magnitude = scaling ? scaling->magnitude : 1.0f;
+    *out = r;
+    return 0;
+}
+
+extern "C" void ojas_b200_rope_destroy(ojas_b200_rope *r) {
+    if (!r) return;
+    DeviceGuard guard(r->ctx->device);
+    cudaFree(r->turns);
+    delete r;
+}
+
+// ---------------------------------------------------------------------------- rows
+struct RopeArgs {
+    const void *x;
+    void *y;
+    const int *pos;
+    const uint64_t *turns;
+    float magnitude;
+    long long x_stride, y_stride;      // elements between tokens
+    long long M;
+    uint32_t x_type, y_type;
+    int heads, dim, rot, tokens_per_cta;
+    bool interleaved;
+};
+
+// One CTA takes tokens_per_cta tokens: it forms their cosines and sines once in shared memory, then every thread owns one
+// unit of a head (VEC pairs, or 2 VEC elements that pass through) and walks the (token, head) rows.
+template <int VEC>
+__global__ void __launch_bounds__(256) rope_rows_kernel(const RopeArgs a) {
+    extern __shared__ float2 rope_cs[];           // [tokens_per_cta][rot / 2]
+    grid_launch_dependents();
+    grid_dependency_wait();                       // x and pos come from the kernels before this one
+    const int half = a.rot >> 1;
+    const long long t0 = (long long)blockIdx.x * a.tokens_per_cta;
+    const int tokens = (int)min((long long)a.tokens_per_cta, a.M - t0);
+    const int tid = threadIdx.y * blockDim.x + threadIdx.x, threads = blockDim.x * blockDim.y;
+    for (int i = tid; i < tokens * half; i += threads) {
+        const int t = i / half, f = i - t * half;
+        rope_cs[i] = rope_angle(__ldg(a.pos + t0 + t), __ldg(a.turns + f), a.magnitude);
+    }
+    __syncthreads();
+    const int units = rope_units(VEC, a.rot, a.dim);
+    for (int u = threadIdx.x; u < units; u += blockDim.x) {
+        const RopeUnit<VEC> unit(u, a.rot, a.dim, a.interleaved);
+        for (int r = threadIdx.y; r < tokens * a.heads; r += blockDim.y) {
+            const int t = r / a.heads, h = r - t * a.heads;
+            const long long xo = (t0 + t) * a.x_stride + (long long)h * a.dim, yo = (t0 + t) * a.y_stride + (long long)h * a.dim;
+            unit.apply(a.x, a.x_type, xo, a.y, a.y_type, yo, rope_cs + t * half);
+        }
+    }
+}
+
+extern "C" int ojas_b200_rope_rows(ojas_b200_ctx *ctx, const ojas_b200_rope *rope, int layout, uint32_t x_type, const void *x, size_t x_stride,
+                                   uint32_t y_type, void *y, size_t y_stride, const int32_t *pos, size_t M, size_t heads, size_t dim) {
+    if (!ctx) return OJAS_B200_E_ARG;
+    if (!rope) return ojas_fail(ctx, OJAS_B200_E_ARG, "rope_rows: null rotation");
+    if (rope->ctx->device != ctx->device) return ojas_fail(ctx, OJAS_B200_E_ARG, "rope_rows: the rotation lives on device %d, the context on %d", rope->ctx->device, ctx->device);
+    char why[256];
+    const int rc = ojas_b200_rope_rows_check(rope->rot_dim, layout, x_type, x, x_stride, y_type, y, y_stride, pos, M, heads, dim, why, sizeof why);
+    if (rc) return ojas_fail(ctx, rc, "%s", why);
+    if (M == 0) return 0;
+    RopeArgs a{};
+    a.x = x; a.y = y; a.pos = pos; a.turns = rope->turns; a.magnitude = rope->magnitude;
+    a.x_stride = (long long)(x_stride ? x_stride : heads * dim);
+    a.y_stride = (long long)(y_stride ? y_stride : heads * dim);
+    a.M = (long long)M; a.x_type = x_type; a.y_type = y_type;
+    a.heads = (int)heads; a.dim = (int)dim; a.rot = (int)rope->rot_dim; a.interleaved = layout == OJAS_B200_ROPE_INTERLEAVED;
+    const bool vec = rope_vec_ok(a.rot, a.dim, a.interleaved) && rope_rows_aligned(x, x_type, a.x_stride) && rope_rows_aligned(y, y_type, a.y_stride);
+    const int units = rope_units(vec ? 4 : 1, a.rot, a.dim);
+    const dim3 block(units < 256 ? units : 256, units < 256 ? 256 / units : 1);
+    // Few tokens: one per CTA, so that all of them run at once; many: several, so that the sines are formed with every lane
+    // busy.  A CTA's angles have to fit in 16 KB.
+    int tpc = M >= (size_t)ctx->sm_count * 16 ? 4 : 1;
+    while (tpc > 1 && tpc * (a.rot / 2) * (int)sizeof(float2) > 16384) tpc >>= 1;
+    a.tokens_per_cta = tpc;
+    const size_t ctas = (M + tpc - 1) / tpc;
+    const size_t smem = (size_t)tpc * (a.rot / 2) * sizeof(float2);
+    DeviceGuard guard(ctx->device);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)ctas); cfg.blockDim = block; cfg.dynamicSmemBytes = smem; cfg.stream = ctx->stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = ctx->pdl ? 1 : 0;
+    const cudaError_t e = vec ? cudaLaunchKernelEx(&cfg, rope_rows_kernel<4>, a) : cudaLaunchKernelEx(&cfg, rope_rows_kernel<1>, a);
+    if (e != cudaSuccess) return ojas_fail(ctx, OJAS_B200_E_CUDA, "launch rope_rows: %s", cudaGetErrorString(e));
+    OJAS_LAUNCH_CHECK(ctx, "rope_rows");
+    return 0;
+}
+
+extern "C" int ojas_b200_rope_rows_check(size_t rot_dim, int layout, uint32_t x_type, const void *x, size_t x_stride, uint32_t y_type, const void *y,
+                                         size_t y_stride, const int32_t *pos, size_t M, size_t heads, size_t dim, char *err, size_t errlen) {
+    auto no = [&](int code, const char *why) { if (err && errlen) snprintf(err, errlen, "rope_rows: %s", why); return code; };
+    if (layout != OJAS_B200_ROPE_HALF && layout != OJAS_B200_ROPE_INTERLEAVED) return no(OJAS_B200_E_ARG, "unknown pair layout");
+    if (!elem_type(x_type) || !elem_type(y_type)) return no(OJAS_B200_E_ARG, "rows must be f32, f16 or bf16");
+    if (heads == 0 || heads > 65536 || dim < 2 || dim > 2048 || dim % 2 != 0) return no(OJAS_B200_E_ARG, "heads must be 1..65536, the head size even, 2..2048");
+    if (rot_dim > dim) return no(OJAS_B200_E_ARG, "the rotated part is larger than a head");
+    if ((x_stride && x_stride < heads * dim) || (y_stride && y_stride < heads * dim)) return no(OJAS_B200_E_ARG, "a row stride is smaller than a row");
+    if (M > 0x3fffffffull || x_stride > (1ull << 40) || y_stride > (1ull << 40)) return no(OJAS_B200_E_LIMIT, "too many rows, or a stride too large");
+    if (M && (!x || !y || !pos)) return no(OJAS_B200_E_ARG, "null pointer");
+    if (M && ((uintptr_t)x % elem_bytes(x_type) || (uintptr_t)y % elem_bytes(y_type) || (uintptr_t)pos % 4)) return no(OJAS_B200_E_ARG, "a pointer is not aligned to its elements");
+    if (M && x == y && (x_type != y_type || (x_stride ? x_stride : heads * dim) != (y_stride ? y_stride : heads * dim)))
+        return no(OJAS_B200_E_ARG, "in place, x and y need the same type and stride");
+    return 0;
+}

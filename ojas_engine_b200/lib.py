@@ -14,6 +14,20 @@ from . import _build
 _vp, _sz, _u32, _u64 = C.c_void_p, C.c_size_t, C.c_uint32, C.c_uint64
 _i = C.c_int
 
+
+
+class RopeScaling(C.Structure):
+    """``ojas_b200_rope_scaling``."""
+    _fields_ = [("factor", C.c_double), ("beta_fast", C.c_double), ("beta_slow", C.c_double), ("orig_len", _sz), ("magnitude", C.c_float)]
+
+
+class SeqsStruct(C.Structure):
+    """``ojas_b200_seqs``."""
+    _fields_ = [("cu", _vp), ("len", _vp), ("table", _vp), ("n_seqs", _sz), ("table_stride", _sz), ("max_rows", _sz), ("max_len", _sz)]
+
+
+_scaling, _seqs, _f = C.POINTER(RopeScaling), C.POINTER(SeqsStruct), C.c_float
+
 # name -> (restype, argtypes); must cover every symbol the header declares
 SIGNATURES = {
     "ojas_b200_create": (_i, [_i, _vp, C.POINTER(_vp)]),
@@ -66,6 +80,20 @@ SIGNATURES = {
     "ojas_b200_moe_workspace_bytes": (_sz, [_sz, _sz, _sz, _sz, _sz]),
     "ojas_b200_moe_ffn": (_i, [_vp, _u32, _u32, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _sz, _vp, _i, _vp, _sz]),
     "ojas_b200_embed_rows": (_i, [_vp, _u32, _vp, _sz, _vp, _sz, _sz, _vp]),
+    "ojas_b200_rope_create": (_i, [_vp, _sz, C.c_double, _scaling, C.POINTER(_f), C.POINTER(_vp)]),
+    "ojas_b200_rope_destroy": (None, [_vp]),
+    "ojas_b200_rope_frequencies": (_i, [_sz, C.c_double, _scaling, C.POINTER(_f), C.POINTER(C.c_double), C.c_char_p, _sz]),
+    "ojas_b200_rope_rows": (_i, [_vp, _vp, _i, _u32, _vp, _sz, _u32, _vp, _sz, _vp, _sz, _sz, _sz]),
+    "ojas_b200_rope_rows_check": (_i, [_sz, _i, _u32, _vp, _sz, _u32, _vp, _sz, _vp, _sz, _sz, _sz, C.c_char_p, _sz]),
+    "ojas_b200_kv_create": (_i, [_vp, _u32, _vp, _vp, _sz, _sz, _sz, _sz, _sz, _sz, _sz, C.POINTER(_vp)]),
+    "ojas_b200_kv_check": (_i, [_u32, _vp, _vp, _sz, _sz, _sz, _sz, _sz, _sz, _sz, C.c_char_p, _sz]),
+    "ojas_b200_kv_destroy": (None, [_vp]),
+    "ojas_b200_seqs_check_host": (_i, [_vp, _vp, _vp, _sz, _sz, _sz, _sz, _sz, _sz, _sz, C.c_char_p, _sz]),
+    "ojas_b200_kv_append": (_i, [_vp, _vp, _seqs, _vp, _i, _u32, _vp, _sz, _vp, _sz, _vp, _sz, _u32, _vp, _sz, _sz, _vp, _sz]),
+    "ojas_b200_kv_append_check": (_i, [_sz, _sz, _sz, _i, _u32, _vp, _sz, _vp, _sz, _vp, _sz, _u32, _vp, _sz, _sz, _vp, _seqs, _sz, C.c_char_p, _sz]),
+    "ojas_b200_attention_workspace_bytes": (_sz, [_vp, _vp, _seqs, _sz, _sz, C.c_longlong]),
+    "ojas_b200_attention": (_i, [_vp, _vp, _seqs, _u32, _vp, _sz, _sz, _f, _i, C.c_longlong, _vp, _sz, _sz, _vp, _sz]),
+    "ojas_b200_attention_check": (_i, [_u32, _sz, _sz, _sz, _u32, _sz, _vp, _sz, _vp, _sz, _f, _i, C.c_longlong, _seqs, _sz, C.c_char_p, _sz]),
     "ojas_b200_gguf_open": (_i, [C.c_char_p, C.POINTER(_vp), C.c_char_p, _sz]),
     "ojas_b200_gguf_close": (None, [_vp]),
     "ojas_b200_gguf_tensor_count": (_sz, [_vp]),

@@ -18,6 +18,8 @@ import numpy as np
 from . import lib as _lib
 
 Q8_0, Q4_K, Q5_K, Q6_K, IQ4_NL, IQ4_XS = 8, 12, 13, 14, 20, 23
+F32, F16, BF16 = 0, 1, 30                      # element types of the operators between the projections
+ROPE_HALF, ROPE_INTERLEAVED = 0, 1
 PLAIN, ACCUM, BIAS = 0, 1, 2
 GEMV_MAX_M = 8
 _TAGS = {Q4_K: "q4k", Q5_K: "q5k", Q6_K: "q6k", Q8_0: "q80", IQ4_NL: "iq4nl", IQ4_XS: "iq4xs"}
@@ -71,6 +73,7 @@ class B200Gpu:
             raise OjasB200Error(rc, f"ojas_b200_create(device={device}) failed: {why}")
         self._ctx = ctx
         self.device = device
+        self._attn_ws: list[Buf] = []
 
     # ------------------------------------------------------------------ plumbing
     def _ck(self, rc: int) -> None:
@@ -274,6 +277,41 @@ class B200Gpu:
         """``x[m, :]`` = the dequantized row ``ids[m]`` of a token table kept as raw GGUF blocks (``q35_embed_q4k``)."""
         self._ck(self._l.ojas_b200_embed_rows(self._ctx, ggml_type, C.c_void_p(table.ptr), rows, C.c_void_p(ids.ptr), m, d, C.c_void_p(x.ptr)))
 
+    # ------------------------------------------------------------------ between the projections
+    def rope_rows(self, rope: Rope, x: Buf, y: Buf, pos: Buf, m: int, heads: int, dim: int, layout: int = ROPE_HALF, x_type: int = F32,
+                  y_type: int = F32, x_stride: int = 0, y_stride: int = 0) -> None:
+        """The heads of x [m, heads, dim] turned by the positions ``pos`` [m] (int32) into y; strides in elements between
+        rows (0: contiguous).  ``y`` may be ``x``."""
+        self._ck(self._l.ojas_b200_rope_rows(self._ctx, rope._h, layout, x_type, x.ptr, x_stride, y_type, y.ptr, y_stride, pos.ptr, m, heads, dim))
+
+    def kv_append(self, kv: KvCache, seqs: Seqs, k: Buf, v: Buf, m: int, rope: Rope | None = None, layout: int = ROPE_HALF, x_type: int = F32,
+                  x_stride: int = 0, q: Buf | None = None, q_out: Buf | None = None, q_heads: int = 0, q_type: int = F32, q_out_stride: int = 0,
+                  pos: Buf | None = None, q_stride: int | None = None, k_stride: int | None = None, v_stride: int | None = None) -> None:
+        """Stores k (rotated) and v of the call's rows at their sequences' newest places in the cache, and q rotated in
+        ``q_out``.  ``x_stride`` is the stride of q, k and v alike (parts of a fused row); each can have its own."""
+        self._ck(self._l.ojas_b200_kv_append(self._ctx, kv._h, seqs._ref, rope._h if rope else None, layout, x_type,
+                                             q.ptr if q else None, x_stride if q_stride is None else q_stride,
+                                             k.ptr, x_stride if k_stride is None else k_stride, v.ptr, x_stride if v_stride is None else v_stride,
+                                             q_type, q_out.ptr if q_out else None, q_out_stride, q_heads, pos.ptr if pos else None, m))
+
+    def attention_workspace_bytes(self, kv: KvCache, seqs: Seqs, m: int, q_heads: int, window: int = 0) -> int:
+        return int(self._l.ojas_b200_attention_workspace_bytes(self._ctx, kv._h, seqs._ref, m, q_heads, window))
+
+    def attention(self, kv: KvCache, seqs: Seqs, q: Buf, out: Buf, m: int, q_heads: int, act_type: int = F32, scale: float | None = None,
+                  causal: bool = True, window: int = 0, q_stride: int = 0, out_stride: int = 0, workspace: Buf | None = None) -> None:
+        """Attention of the call's rows over their sequences' keys (scale: 1 / sqrt(dim) unless given).  Without a caller
+        workspace a grow-only scratch buffer owned by this object is used; a buffer it outgrew stays allocated, because a
+        captured graph may still use it."""
+        need = self._l.ojas_b200_attention_workspace_bytes(self._ctx, kv._h, seqs._ref, m, q_heads, window)
+        if workspace is None and need:
+            workspace = self._attn_ws[-1] if self._attn_ws else None
+            if workspace is None or workspace.nbytes < need:
+                workspace = self.alloc_bytes(max(need, 2 * workspace.nbytes if workspace else 0))
+                self._attn_ws.append(workspace)
+        self._ck(self._l.ojas_b200_attention(self._ctx, kv._h, seqs._ref, act_type, q.ptr, q_stride, q_heads, kv.dim ** -0.5 if scale is None else scale,
+                                             1 if causal else 0, window, out.ptr, out_stride, m, workspace.ptr if workspace else None,
+                                             workspace.nbytes if workspace else 0))
+
     def gemv_idots(self, w: Lin, x: Buf, idots: Buf) -> None:
         self._ck(self._l.ojas_b200_gemv_idots(self._ctx, w.ggml_type, C.c_void_p(x.ptr), C.c_void_p(w.buf.ptr), C.c_void_p(idots.ptr), w.k, w.n))
 
@@ -347,6 +385,86 @@ class B200Gpu:
         raw = (C.c_uint8 * nbytes).from_address(p.value)
         arr = np.frombuffer(raw, dtype=np.uint8).view(dtype)
         return arr
+
+
+class Rope:
+    """The rotation of a model's heads: frequencies base^(-2i / rot_dim), scaled for long contexts (``ojas_b200_rope_create``
+    has the formulas).  ``freq_factors``: one divisor per pair, as a GGUF file's rope_freqs tensor holds them."""
+
+    def __init__(self, gpu: B200Gpu, rot_dim: int, base: float = 10000.0, factor: float = 1.0, orig_len: int = 0, beta_fast: float = 32.0,
+                 beta_slow: float = 1.0, magnitude: float = 1.0, freq_factors=None):
+        self.gpu, self._l, self.rot_dim = gpu, gpu._l, rot_dim
+        self._h = None
+        h = C.c_void_p()
+        gpu._ck(self._l.ojas_b200_rope_create(gpu.ctx, rot_dim, base, *_rope_arguments(rot_dim, factor, orig_len, beta_fast, beta_slow, magnitude, freq_factors),
+                                              C.byref(h)))
+        self._h = h
+
+    def close(self) -> None:
+        if getattr(self, "_h", None) and self.gpu._ctx:
+            self._l.ojas_b200_rope_destroy(self._h)
+        self._h = None
+
+    def __del__(self):  # pragma: no cover
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def _rope_arguments(rot_dim, factor, orig_len, beta_fast, beta_slow, magnitude, freq_factors):
+    scaling = _lib.RopeScaling(factor, beta_fast, beta_slow, orig_len, magnitude)
+    ff = None
+    if freq_factors is not None:
+        ff = np.ascontiguousarray(freq_factors, np.float32)
+        if ff.size != rot_dim // 2:
+            raise OjasB200Error(-1, f"rope: {ff.size} frequency factors for {rot_dim // 2} pairs")
+        ff = (C.c_float * ff.size)(*ff.tolist())
+    return C.byref(scaling), ff
+
+
+class KvCache:
+    """Describes a paged cache in the caller's buffers k and v: [pages][heads][page_size][dim] values unless strides (in
+    elements) say otherwise."""
+
+    def __init__(self, gpu: B200Gpu, ggml_type: int, k: Buf, v: Buf, pages: int, page_size: int, heads: int, dim: int, page_stride: int | None = None,
+                 head_stride: int | None = None, token_stride: int | None = None):
+        self.gpu, self._l = gpu, gpu._l
+        self._h = None
+        self.type, self.k, self.v, self.pages, self.page_size, self.heads, self.dim = ggml_type, k, v, pages, page_size, heads, dim
+        self.page_stride = heads * page_size * dim if page_stride is None else page_stride
+        self.head_stride = page_size * dim if head_stride is None else head_stride
+        self.token_stride = dim if token_stride is None else token_stride
+        need = 2 * ((pages - 1) * self.page_stride + (heads - 1) * self.head_stride + (page_size - 1) * self.token_stride + dim)
+        if min(k.nbytes, v.nbytes) < need:
+            raise OjasB200Error(-1, f"KvCache: buffers of {k.nbytes} and {v.nbytes} bytes, {need} needed")
+        h = C.c_void_p()
+        gpu._ck(self._l.ojas_b200_kv_create(gpu.ctx, ggml_type, k.ptr, v.ptr, pages, page_size, heads, dim, self.page_stride, self.head_stride,
+                                            self.token_stride, C.byref(h)))
+        self._h = h
+
+    def close(self) -> None:
+        if getattr(self, "_h", None):
+            self._l.ojas_b200_kv_destroy(self._h)
+        self._h = None
+
+    def __del__(self):  # pragma: no cover
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class Seqs:
+    """A batch of sequences for ``kv_append`` and ``attention``: device arrays cu [n + 1], len [n], table [n, table_stride]
+    (int32; see ``ojas_b200_seqs``) and host bounds on new rows and length."""
+
+    def __init__(self, cu: Buf, lens: Buf, table: Buf, n_seqs: int, table_stride: int, max_rows: int, max_len: int):
+        if cu.nbytes < 4 * (n_seqs + 1) or lens.nbytes < 4 * n_seqs or table.nbytes < 4 * n_seqs * table_stride:
+            raise OjasB200Error(-1, "Seqs: a buffer is smaller than its array")
+        self.cu, self.lens, self.table = cu, lens, table
+        self._struct = _lib.SeqsStruct(cu.ptr, lens.ptr, table.ptr, n_seqs, table_stride, max_rows, max_len)
+        self._ref = C.byref(self._struct)
 
 
 class ExpertCache:
@@ -432,6 +550,18 @@ def encode(ggml_type: int, w: np.ndarray) -> np.ndarray:
     rc = _lib.load().ojas_b200_encode_host(ggml_type, w.ctypes.data_as(C.c_void_p), n, k, out.ctypes.data_as(C.c_void_p))
     if rc != 0:
         raise OjasB200Error(rc, f"encode: type {ggml_type} [{n},{k}]")
+    return out
+
+
+def rope_frequencies(rot_dim: int, base: float = 10000.0, factor: float = 1.0, orig_len: int = 0, beta_fast: float = 32.0, beta_slow: float = 1.0,
+                     magnitude: float = 1.0, freq_factors=None) -> np.ndarray:
+    """The frequencies (radians per position) a ``Rope`` of these arguments turns by."""
+    out = np.empty(max(rot_dim // 2, 1), np.float64)
+    err = C.create_string_buffer(256)
+    rc = _lib.load().ojas_b200_rope_frequencies(rot_dim, base, *_rope_arguments(rot_dim, factor, orig_len, beta_fast, beta_slow, magnitude, freq_factors),
+                                                out.ctypes.data_as(C.POINTER(C.c_double)), err, 256)
+    if rc != 0:
+        raise OjasB200Error(rc, err.value.decode())
     return out
 
 

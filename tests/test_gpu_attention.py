@@ -1,0 +1,418 @@
+"""Rotary positions, the append to a paged cache and attention over it on the GPU, against their plain forms in 64 bits.
+Tolerances are the roundings an evaluation makes, counted (tests/attn_helpers.py)."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import ojas_engine_b200 as ob
+from attn_helpers import HALF, TORCH, Batch, attention_bound, buf, check, rope_bound, rope_exact
+
+pytestmark = pytest.mark.gpu
+F32, F16, BF16 = ob.F32, ob.F16, ob.BF16
+HALVES, INTER = ob.ROPE_HALF, ob.ROPE_INTERLEAVED
+
+
+def randn(g, *shape, dtype=torch.float32):
+    return torch.randn(*shape, generator=g).to(dtype)
+
+
+# ------------------------------------------------------------------------------------------------------------------ rope
+@pytest.mark.parametrize("layout", [HALVES, INTER])
+@pytest.mark.parametrize("tokens,heads,dim,rot,xt,yt", [
+    (1, 1, 64, 64, F32, F32), (7, 5, 128, 128, F32, F16), (33, 3, 256, 64, F32, BF16), (5, 9, 128, 96, F16, F16), (3, 2, 80, 80, BF16, F32),
+    (2, 3, 6, 4, F32, F32), (9, 2, 130, 10, F16, F32), (1, 1, 2, 2, F32, F32), (2, 1, 2048, 1024, F32, F32), (2500, 4, 64, 32, F32, BF16)])
+def test_rope_rows(gpu, layout, tokens, heads, dim, rot, xt, yt):
+    g = torch.Generator().manual_seed(tokens + dim)
+    x = randn(g, tokens, heads, dim, dtype=TORCH[xt])
+    pos = torch.randint(-(2 ** 31), 2 ** 31 - 1, (tokens,), generator=g, dtype=torch.int64).to(torch.int32)
+    pos[0] = 0 if tokens > 1 else 1000003
+    rope = ob.Rope(gpu, rot, base=10000.0)
+    xd, pd, yd = x.cuda(), pos.cuda(), torch.full((tokens + 2, heads, dim), 77.0, dtype=TORCH[yt]).cuda()
+    torch.cuda.synchronize()
+    gpu.rope_rows(rope, buf(xd), buf(yd), buf(pd), tokens, heads, dim, layout=layout, x_type=xt, y_type=yt)
+    gpu.sync()
+    # positions of 31 bits: the angle has to be reduced exactly, here with integers
+    turns = [int(math.floor(math.ldexp(f / (2 * math.pi), 64))) for f in ob.rope_frequencies(rot)]
+    frac = torch.tensor([[((int(p) * t) % (1 << 64)) / 2.0 ** 64 for t in turns] for p in pos], dtype=torch.float64)
+    one = rope_exact(x, torch.ones(tokens), np.zeros(rot // 2), layout)     # shape and the passing part
+    a, b = (x[..., : rot // 2].double(), x[..., rot // 2 : rot].double()) if layout == HALVES else (x[..., 0:rot:2].double(), x[..., 1:rot:2].double())
+    c, s = torch.cos(2 * math.pi * frac)[:, None], torch.sin(2 * math.pi * frac)[:, None]
+    u, v = a * c - b * s, b * c + a * s
+    if layout == HALVES:
+        one[..., : rot // 2], one[..., rot // 2 : rot] = u, v
+    else:
+        one[..., 0:rot:2], one[..., 1:rot:2] = u, v
+    check(yd[:tokens], one, rope_bound(x, one, rot, layout, 1.0, yt))
+    assert (yd[tokens:] == 77).all()
+
+
+@pytest.mark.parametrize("layout", [HALVES, INTER])
+def test_rope_scaled_strided_and_in_place(gpu, layout):
+    """Heads inside a fused row, frequencies scaled by parts, in place: the other heads of the row keep their values; and back."""
+    g = torch.Generator().manual_seed(3)
+    tokens, heads, fused, dim, rot = 19, 6, 11, 128, 64
+    x = randn(g, tokens, fused, dim)
+    pos = torch.randint(0, 100000, (tokens,), generator=g).to(torch.int32)
+    kw = dict(base=500000.0, factor=8.0, orig_len=8192, beta_fast=4.0, beta_slow=1.0, magnitude=1.25)
+    rope, freq = ob.Rope(gpu, rot, **kw), ob.rope_frequencies(rot, **kw)
+    xd, pd, back = x.cuda(), pos.cuda(), (-pos).cuda()
+    torch.cuda.synchronize()
+    first = ob.Buf(buf(xd).ptr + 2 * dim * 4, buf(xd).nbytes - 2 * dim * 4)   # heads 2..7 of each row
+    gpu.rope_rows(rope, first, first, buf(pd), tokens, heads, dim, layout=layout, x_stride=fused * dim, y_stride=fused * dim)
+    gpu.sync()
+    want = rope_exact(x[:, 2:8], pos, freq, layout, 1.25)
+    check(xd[:, 2:8], want, rope_bound(x[:, 2:8], want, rot, layout, 1.25, F32) + 1.25 * 2.0 ** -30)
+    assert torch.equal(xd[:, :2].cpu(), x[:, :2]) and torch.equal(xd[:, 8:].cpu(), x[:, 8:])
+    gpu.rope_rows(rope, first, first, buf(back), tokens, heads, dim, layout=layout, x_stride=fused * dim, y_stride=fused * dim)
+    gpu.sync()
+    assert (xd[:, 2:8, :rot].cpu() - x[:, 2:8, :rot] * 1.25 ** 2).abs().max() < 6 * 1.25 ** 2 * 2.0 ** -20   # two rotations of values below 6
+
+
+# ---------------------------------------------------------------------------------------------------------------- append
+@pytest.mark.parametrize("layout,rot", [(HALVES, 128), (INTER, 128), (INTER, 32), (HALVES, 0)])
+@pytest.mark.parametrize("xt,ct,qt,page,nhd", [(F32, F16, F32, 16, False), (F32, BF16, BF16, 48, True), (F16, F16, F16, 64, False), (BF16, BF16, F32, 16, True)])
+def test_append(gpu, layout, rot, xt, ct, qt, page, nhd):
+    """Ragged rows, a sequence with none, rows behind the last sequence; every cache value that is not appended stays."""
+    hq, hk, dim = 6, 2, 128
+    b = Batch(rows=[3, 0, 17, 1, 40], lens=[3, 5, 100, 48, 41], kv_heads=hk, dim=dim, page=page, cache=ct, nhd=nhd, seed=rot + page, extra_rows=3).upload(gpu)
+    g = torch.Generator().manual_seed(5)
+    x = randn(g, b.M, hq + 2 * hk, dim, dtype=TORCH[xt])
+    xd, qo = x.cuda(), torch.full((b.M, hq, dim), 77.0, dtype=TORCH[qt]).cuda()
+    rope = ob.Rope(gpu, rot, base=10000.0, magnitude=1.5) if rot else None
+    base, size = buf(xd), dim * xd.element_size()
+    q, k, v = (ob.Buf(base.ptr + n * size, base.nbytes - n * size) for n in (0, hq, hq + hk))
+    torch.cuda.synchronize()
+    gpu.kv_append(b.kv, b.seqs, k, v, b.M, rope=rope, layout=layout, x_type=xt, x_stride=(hq + 2 * hk) * dim, q=q, q_out=buf(qo), q_heads=hq, q_type=qt)
+    gpu.sync()
+    freq = ob.rope_frequencies(rot) if rot else np.zeros(0)
+    want_k, want_v = b.k.double(), b.v.double()
+    bound = torch.zeros_like(want_k)
+    for i, (n, total) in enumerate(zip(b.rows, b.lens)):
+        t0, pos = int(b.cu[i]), torch.arange(total - n, total)
+        rows = x[t0 : t0 + n]
+        turn = (lambda h: rope_exact(h, pos, freq, layout, 1.5)) if rot else (lambda h: h.double())
+        err = (lambda h, y, t: rope_bound(h, y, rot, layout, 1.5, t)) if rot else (lambda h, y, t: HALF[t] * y.abs() + 2.0 ** -25)
+        wq, wk = turn(rows[:, :hq]), turn(rows[:, hq : hq + hk])
+        if n:
+            check(qo[t0 : t0 + n], wq, err(rows[:, :hq], wq, qt), f"q of sequence {i}")
+        b.put(want_k, i, total - n, wk)
+        b.put(want_v, i, total - n, rows[:, hq + hk :].to(TORCH[ct]).double())
+        b.put(bound, i, total - n, err(rows[:, hq : hq + hk], wk, ct))
+    got_k, got_v = b.dev["k"].double().cpu(), b.dev["v"].double().cpu()
+    assert torch.equal(torch.isnan(got_k), torch.isnan(want_k)) and torch.equal(got_v.nan_to_num(nan=9.9), want_v.nan_to_num(nan=9.9))
+    assert ((got_k - want_k).abs().nan_to_num(nan=0.0) <= bound).all()
+    assert (qo[int(b.cu[-1]) :] == 77).all()
+
+
+def test_append_positions_and_no_query(gpu):
+    """Positions of their own (a cache whose tokens were moved), no query rows, unaligned rows: the element-by-element form."""
+    b = Batch(rows=[2, 5], lens=[20, 5], kv_heads=1, dim=64, page=16, seed=1).upload(gpu)
+    g = torch.Generator().manual_seed(9)
+    x = randn(g, b.M, 131)
+    pos = torch.tensor([5, 70000, 1, 2, 3, -4, 1 << 30], dtype=torch.int32)
+    xd, pd, rope = x.cuda(), pos.cuda(), ob.Rope(gpu, 64)
+    base = buf(xd)
+    torch.cuda.synchronize()
+    gpu.kv_append(b.kv, b.seqs, ob.Buf(base.ptr + 4, 0), ob.Buf(base.ptr + 4 * 66, 0), b.M, rope=rope, x_stride=131, pos=buf(pd))
+    gpu.sync()
+    turns = [int(math.floor(math.ldexp(f / (2 * math.pi), 64))) for f in ob.rope_frequencies(64)]
+    k = x[:, 1:65].view(-1, 1, 64)
+    frac = torch.tensor([[((int(p) * t) % (1 << 64)) / 2.0 ** 64 for t in turns] for p in pos], dtype=torch.float64)[:, None]
+    c, s = torch.cos(2 * math.pi * frac), torch.sin(2 * math.pi * frac)
+    want = torch.cat([k[..., :32] * c - k[..., 32:] * s, k[..., 32:] * c + k[..., :32] * s], -1)
+    at = [(0, 18), (0, 19)] + [(1, i) for i in range(5)]
+    got = torch.stack([b.view(b.dev["k"].cpu())[b.table[i, p // 16], p % 16] for i, p in at])
+    check(got, want, rope_bound(k, want, 64, HALVES, 1.0, F16))
+    got = torch.stack([b.view(b.dev["v"].cpu())[b.table[i, p // 16], p % 16] for i, p in at])
+    assert torch.equal(got[:, 0], x[:, 66:130].half())
+
+
+# ------------------------------------------------------------------------------------------------------------- attention
+def run_attention(gpu, b, hq, act, causal=True, window=0, scale=None, seed=3, q_scale=1.0, p_terms=None, stride=0, workspace=None):
+    q = (randn(torch.Generator().manual_seed(seed), b.M, hq, b.dim) * q_scale).to(TORCH[act])
+    qd = torch.full((b.M, stride or hq * b.dim), 5.0, dtype=TORCH[act]).cuda()
+    qd[:, : hq * b.dim] = q.reshape(b.M, -1).cuda()
+    out = torch.full_like(qd, 77.0)
+    torch.cuda.synchronize()
+    gpu.attention(b.kv, b.seqs, buf(qd), buf(out), b.M, hq, act_type=act, causal=causal, window=window, scale=scale, q_stride=stride, out_stride=stride, workspace=workspace)
+    gpu.sync()
+    want, weight, vmax = b.attention_exact(q, hq, scale=scale, causal=causal, window=window, fill=77.0)
+    bound = attention_bound(want, weight, vmax, b.dim, max(b.lens), act, b.cache, p_terms or (2 if act == F32 else 1))
+    got = out[:, : hq * b.dim].reshape(b.M, hq, b.dim)
+    assert (out[:, hq * b.dim :] == 77).all()
+    check(got, want, bound)
+    first, last = int(b.cu[0]), int(b.cu[-1])
+    assert (got[last:] == 77).all() and (got[:first] == 77).all()
+    return out
+
+
+TYPES = [(F32, F16), (F16, F16), (BF16, BF16), (F32, BF16)]
+
+
+@pytest.mark.parametrize("act,cache", TYPES)
+@pytest.mark.parametrize("dim,group,page,nhd", [(64, 1, 16, False), (128, 8, 16, True), (128, 3, 48, False), (256, 4, 64, True), (128, 16, 128, False), (64, 7, 256, True), (256, 20, 32, False)])
+def test_decode(gpu, act, cache, dim, group, page, nhd):
+    """One new token per sequence: lengths of one, around a block and a page, and long enough to be split; one sequence without
+    a new row and one without any token."""
+    lens = [1, 2, 15, 16, 17, 63, 64, 65, 0, 127, 129, 700, 1500]
+    rows = [1] * 8 + [0, 1, 0, 1, 1]
+    b = Batch(rows, lens, kv_heads=2, dim=dim, page=page, cache=cache, nhd=nhd, seed=dim + group, extra_rows=2).upload(gpu)
+    run_attention(gpu, b, 2 * group, act)
+
+
+@pytest.mark.parametrize("act,cache", TYPES)
+@pytest.mark.parametrize("dim,group,rows,window", [(128, 4, [5, 1, 33, 0, 128], 0), (64, 2, [64, 63, 65, 1], 0), (128, 7, [40, 100], 50), (256, 4, [9, 30], 0),
+                                                   (64, 5, [200], 16), (128, 1, [300, 2], 1), (256, 1, [130, 1, 1], 100)])
+def test_chunk(gpu, act, cache, dim, group, rows, window):
+    """Several new tokens over what is in the cache: some from their sequence's start, some behind a long beginning."""
+    lens = [n + (0, 1, 77, 300)[i % 4] for i, n in enumerate(rows)]
+    b = Batch(rows, lens, kv_heads=2, dim=dim, page=16 if window else 32, cache=cache, seed=dim + group, extra_rows=1).upload(gpu)
+    run_attention(gpu, b, 2 * group, act, window=window)
+
+
+@pytest.mark.parametrize("act,cache", [(F32, F16), (BF16, BF16)])
+@pytest.mark.parametrize("rows", [[1, 1], [20, 150]])
+def test_all_keys(gpu, act, cache, rows):
+    """Not causal: every row sees the whole sequence."""
+    b = Batch(rows, [200, 333], kv_heads=2, dim=128, cache=cache, seed=8).upload(gpu)
+    run_attention(gpu, b, 8, act, causal=False)
+
+
+@pytest.mark.parametrize("act,cache", [(F32, F16), (F16, F16)])
+@pytest.mark.parametrize("rows", [1, 4, 200])
+def test_rows_that_see_nothing(gpu, act, cache, rows):
+    """A sequence shorter than its new rows: the first rows see no key and give zeros, the call is reported."""
+    b = Batch([rows, rows], [rows, rows], kv_heads=1, dim=128, seed=1).upload(gpu)
+    b.dev["len"].copy_(torch.tensor([rows // 2, 0], dtype=torch.int32))
+    q = randn(torch.Generator().manual_seed(1), 2 * rows, 4, 128, dtype=TORCH[act]).cuda()
+    out = torch.full_like(q, 77.0)
+    torch.cuda.synchronize()
+    gpu.attention(b.kv, b.seqs, buf(q), buf(out), 2 * rows, 4, act_type=act)
+    with pytest.raises(ob.OjasB200Error) as e:
+        gpu.sync()
+    assert e.value.code == -5 and "batch" in str(e.value)
+    torch.cuda.synchronize()
+    assert (out[: rows - rows // 2] == 0).all() and (out[rows:] == 0).all()
+    assert torch.isfinite(out).all() and not (out == 77).any()
+
+
+@pytest.mark.parametrize("rows", [1, 60])
+def test_a_window_leaves_old_pages_alone(gpu, rows):
+    """Pages wholly in front of the window may be gone: their table entries are -1 here."""
+    b = Batch([rows], [900], kv_heads=2, dim=128, page=16, seed=4)
+    first = (900 - rows - 100 + 1) // 16
+    b.table[0, :first] = -1
+    b.upload(gpu)
+    run_attention(gpu, b, 8, F32, window=100)
+
+
+@pytest.mark.parametrize("rows,dim", [(1, 128), (30, 128), (1, 256), (100, 64)])
+def test_bad_pages_read_as_zeros_and_are_reported(gpu, rows, dim):
+    b = Batch([rows], [300], kv_heads=2, dim=dim, page=16, seed=4)
+    good = b.table.clone()
+    b.upload(gpu)
+    b.dev["table"][0, 3], b.dev["table"][0, 9] = -7, 1 << 30
+    for i in (3, 9):
+        b.k_rows[0][16 * i : 16 * i + 16] = 0
+        b.v_rows[0][16 * i : 16 * i + 16] = 0
+    with pytest.raises(ob.OjasB200Error) as e:
+        run_attention(gpu, b, 4, F32)
+    assert e.value.code == -5
+    # the same call again: nothing was lost, and without the error its result is that of zero pages
+    q = randn(torch.Generator().manual_seed(3), b.M, 4, dim)
+    qd, out = q.cuda(), torch.full((b.M, 4, dim), 77.0).cuda()
+    torch.cuda.synchronize()
+    gpu.attention(b.kv, b.seqs, buf(qd), buf(out), b.M, 4)
+    torch.cuda.synchronize()
+    want, weight, vmax = b.attention_exact(q, 4)
+    check(out, want, attention_bound(want, weight, vmax, dim, 300, F32, F16, 2))
+    with pytest.raises(ob.OjasB200Error):
+        gpu.sync()
+    x, rope = torch.randn(b.M, 3, dim).cuda(), ob.Rope(gpu, dim)
+    b.dev["table"].copy_(good)
+    b.dev["table"][0, 299 // 16] = b.pages
+    before = b.dev["k"].clone()
+    p = buf(x)
+    torch.cuda.synchronize()
+    gpu.kv_append(b.kv, b.seqs, p, p, 1 if rows == 1 else b.M, rope=rope, x_stride=3 * dim)
+    with pytest.raises(ob.OjasB200Error) as e:
+        gpu.sync()
+    assert e.value.code == -5
+    changed = (b.view(b.dev["k"]).nan_to_num(nan=9.0) != b.view(before).nan_to_num(nan=9.0)).flatten(2).any(-1).sum().item()
+    assert changed == rows - min(rows, 300 - 299 // 16 * 16)
+
+
+@pytest.mark.parametrize("act,cache", TYPES)
+def test_large_scores_and_values(gpu, act, cache):
+    """Scores of some hundreds (one key takes all), and f16 values near the type's limit."""
+    b = Batch([1, 40], [500, 260], kv_heads=2, dim=128, cache=cache, seed=6)
+    for v in b.v_rows:
+        v.mul_(8000.0 if cache == F16 else 1e30)
+    for i in range(2):
+        b.put(b.v, i, 0, b.v_rows[i])
+    b.upload(gpu)
+    run_attention(gpu, b, 8, act, q_scale=40.0)
+    if act == F32:
+        run_attention(gpu, b, 8, act, q_scale=1e6, scale=1e-6)     # beyond f16's range before the scale
+        run_attention(gpu, b, 8, act, q_scale=1e-9, scale=1e8)
+
+
+def test_strides_between_rows(gpu):
+    b = Batch([3, 70], [40, 200], kv_heads=2, dim=64, seed=2).upload(gpu)
+    run_attention(gpu, b, 6, F32, stride=6 * 64 + 20)
+    b = Batch([1, 1], [40, 200], kv_heads=2, dim=128, cache=BF16, seed=2).upload(gpu)
+    run_attention(gpu, b, 4, BF16, stride=4 * 128 + 4)
+
+
+def test_many_sequences(gpu):
+    """More sequences than a warp has lanes, most of them short; rows that begin behind the call's first."""
+    g = torch.Generator().manual_seed(1)
+    n = 150
+    lens = torch.randint(1, 90, (n,), generator=g).tolist()
+    rows = [min(l, int(r)) for l, r in zip(lens, torch.randint(0, 4, (n,), generator=g))]
+    b = Batch(rows, lens, kv_heads=1, dim=64, seed=2, extra_rows=5)
+    b.cu += 3
+    b.M += 3
+    b.upload(gpu)
+    run_attention(gpu, b, 4, F32)
+    b = Batch([1] * n, lens, kv_heads=1, dim=64, seed=2).upload(gpu)
+    x, qo = torch.randn(n, 6, 64).cuda(), torch.zeros(n, 4, 64).cuda()
+    p = buf(x)
+    torch.cuda.synchronize()
+    gpu.kv_append(b.kv, b.seqs, ob.Buf(p.ptr + 4 * 256, 0), ob.Buf(p.ptr + 4 * 320, 0), n, x_stride=384, q=p, q_out=buf(qo), q_heads=4)
+    gpu.sync()
+    assert torch.equal(qo, x[:, :4])
+    k = b.view(b.dev["k"].cpu())
+    for i in range(n):
+        assert torch.equal(k[b.table[i, (lens[i] - 1) // 16], (lens[i] - 1) % 16, 0], x[i, 4].half().cpu())
+
+
+def test_bounds_larger_than_the_batch(gpu):
+    """max_rows and max_len are bounds, not values."""
+    for rows, max_rows, max_len in (([1, 1], 1, 100000), ([3, 2], 500, 600), ([1, 64], 64, 50000)):
+        b = Batch(rows, [333, 90], kv_heads=2, dim=128, seed=2, max_rows=max_rows, max_len=max_len).upload(gpu)
+        run_attention(gpu, b, 8, F32)
+
+
+def test_workspace_is_checked(gpu):
+    b = Batch([1], [4000], kv_heads=2, dim=128, seed=2).upload(gpu)
+    need = gpu.attention_workspace_bytes(b.kv, b.seqs, 1, 8)
+    assert need > 0
+    q, out, ws = torch.zeros(8, 128).cuda(), torch.zeros(8, 128).cuda(), torch.zeros(need + 256, dtype=torch.uint8).cuda()
+    for size, shift in ((need - 1, 0), (need, 8)):
+        with pytest.raises(ob.OjasB200Error) as e:
+            gpu.attention(b.kv, b.seqs, buf(q), buf(out), 1, 8, workspace=ob.Buf(ws.data_ptr() + shift, size))
+        assert e.value.code == -1
+    run_attention(gpu, b, 8, F32, workspace=ob.Buf(ws.data_ptr(), need))
+
+
+@pytest.mark.parametrize("rows", [1, 50])
+def test_captured_and_replayed(gpu, rows):
+    """Append and attention in a graph: the batch's arrays are read at replay, so one graph serves growing sequences; two graphs
+    share the workspace in turn; results do not change from run to run."""
+    b = Batch([rows, rows], [600, 350], kv_heads=2, dim=128, page=16, seed=5, max_len=700)
+    b.upload(gpu)
+    hq, rope = 8, ob.Rope(gpu, 128)
+    x = torch.randn(2 * rows, hq + 4, 128).cuda()
+    q, out = torch.empty(2 * rows, hq, 128).cuda(), torch.empty(2 * rows, hq, 128).cuda()
+    p, width = buf(x), 4 * 128
+
+    def step():
+        gpu.kv_append(b.kv, b.seqs, ob.Buf(p.ptr + hq * width, 0), ob.Buf(p.ptr + (hq + 2) * width, 0), 2 * rows, rope=rope, x_stride=(hq + 4) * 128, q=p,
+                      q_out=buf(q), q_heads=hq)
+        gpu.attention(b.kv, b.seqs, buf(q), buf(out), 2 * rows, hq)
+
+    torch.cuda.synchronize()
+    step()
+    gpu.sync()
+    graphs = []
+    for _ in range(2):
+        gpu.graph_begin()
+        step()
+        graphs.append(gpu.graph_end())
+    for lens in ([600, 350], [601, 340], [rows, 608]):
+        b.dev["len"].copy_(torch.tensor(lens, dtype=torch.int32))
+        torch.cuda.synchronize()
+        results = []
+        for run in (step, lambda: gpu.graph_launch(graphs[0]), lambda: gpu.graph_launch(graphs[1])):
+            out.fill_(0)
+            torch.cuda.synchronize()
+            run()
+            run()
+            try:
+                gpu.sync()
+            except ob.OjasB200Error:
+                pytest.fail("the batch was refused")
+            results.append(out.clone())
+        assert torch.equal(results[0], results[1]) and torch.equal(results[0], results[2])
+    for gr in graphs:
+        gpu.graph_destroy(gr)
+
+
+def test_another_stream_and_context(gpu):
+    """A second context on torch's stream: the handles serve both."""
+    side = torch.cuda.Stream()
+    other = ob.B200Gpu(0, stream=side.cuda_stream)
+    b = Batch([1, 90], [300, 200], kv_heads=2, dim=128, seed=5).upload(gpu)
+    q = randn(torch.Generator().manual_seed(3), b.M, 8, 128)
+    with torch.cuda.stream(side):
+        qd, out = q.cuda(), torch.empty(b.M, 8, 128, device="cuda")
+        other.attention(b.kv, b.seqs, buf(qd), buf(out), b.M, 8)
+        got = out.cpu()
+    want, weight, vmax = b.attention_exact(q, 8)
+    check(got, want, attention_bound(want, weight, vmax, 128, 300, F32, F16, 2))
+    other.close()
+
+
+def test_a_layer_from_its_input_to_the_output_projection(gpu):
+    """Norm + fused QKV projection, append, attention, output projection: a prompt of 70 tokens in two chunks and four single
+    tokens, against the same steps in 64 bits with the framework's own projections taken as they are."""
+    d, hq, hk, dim = 512, 8, 2, 64
+    rng = np.random.default_rng(0)
+    wqkv, wo = (rng.standard_normal((n, d), dtype=np.float32) * np.float32(0.05) for n in ((hq + 2 * hk) * dim, d))
+    lin, lo = (gpu.load_weight(ob.encode(ob.Q6_K, w), ob.Q6_K, w.shape[0], d) for w in (wqkv, wo))
+    b = Batch([0], [74], kv_heads=hk, dim=dim, page=16, seed=5, max_rows=64)
+    b.k.fill_(math.nan)
+    b.v.fill_(math.nan)
+    b.upload(gpu)
+    rope, freq = ob.Rope(gpu, 32, base=10000.0), ob.rope_frequencies(32)
+    done, keys, values = 0, [], []
+    for n in (64, 6, 1, 1, 1, 1):
+        x = gpu.upload(rng.standard_normal((n, d), dtype=np.float32))
+        width = (hq + 2 * hk) * dim
+        qkv, q, att, y = gpu.alloc(n * width), gpu.alloc(n * d), gpu.alloc(n * d), gpu.alloc(n * d)
+        b.dev["cu"].copy_(torch.tensor([0, n], dtype=torch.int32))
+        b.dev["len"].fill_(done + n)
+        torch.cuda.synchronize()
+        gpu.mm(x, lin, qkv, n)
+        gpu.kv_append(b.kv, b.seqs, qkv_part(qkv, hq * dim), qkv_part(qkv, (hq + hk) * dim), n, rope=rope, layout=INTER, x_stride=width, q=qkv, q_out=q, q_heads=hq)
+        gpu.attention(b.kv, b.seqs, q, att, n, hq)
+        gpu.mm(att, lo, y, n)
+        rows = torch.from_numpy(gpu.read(qkv, np.float32, n * width).reshape(n, hq + 2 * hk, dim))
+        pos = torch.arange(done, done + n)
+        keys.append(rope_exact(rows[:, hq : hq + hk], pos, freq, INTER))
+        values.append(rows[:, hq + hk :].double())
+        k, v = (torch.cat(t).repeat_interleave(hq // hk, 1).transpose(0, 1) for t in (keys, values))
+        s = rope_exact(rows[:, :hq], pos, freq, INTER).transpose(0, 1) @ k.transpose(1, 2) * dim ** -0.5
+        s.masked_fill_(torch.arange(done + n) > pos[:, None], -math.inf)
+        want = (torch.softmax(s, -1) @ v).transpose(0, 1).reshape(n, d)
+        got = torch.from_numpy(gpu.read(att, np.float32, n * d).reshape(n, d)).double()
+        # keys and values are rounded to f16 once: 2^-11 of a score's size and of a value
+        size = (rope_exact(rows[:, :hq], pos, freq, INTER).abs().transpose(0, 1) @ k.abs().transpose(1, 2) * dim ** -0.5).max().item()
+        assert (got - want).abs().max().item() <= (2 * size + 1) * 2.0 ** -11 * v.abs().max().item() * 1.05
+        back = gpu.alloc(n * d)
+        again = gpu.upload(got.numpy().astype(np.float32))
+        gpu.mm(again, lo, back, n)
+        a, c = gpu.read(y, np.float32, n * d), gpu.read(back, np.float32, n * d)
+        assert np.linalg.norm(a - c) <= 1e-5 * np.linalg.norm(c)          # the projection read what attention wrote
+        done += n
+        for t in (x, qkv, q, att, y, back, again):
+            gpu.free(t)
+    for t in (lin.buf, lo.buf):
+        gpu.free(t)
+
+
+def qkv_part(b, floats):
+    return ob.Buf(b.ptr + 4 * floats, b.nbytes - 4 * floats)
