@@ -341,12 +341,14 @@ def test_captured_and_replayed(gpu, rows):
             torch.cuda.synchronize()
             run()
             run()
-            try:
+            if lens[1] <= 350:
                 gpu.sync()
-            except ob.OjasB200Error:
-                pytest.fail("the batch was refused")
+            else:                                      # longer than its pages: reported, and the same zeros every time
+                with pytest.raises(ob.OjasB200Error):
+                    gpu.sync()
             results.append(out.clone())
-        assert torch.equal(results[0], results[1]) and torch.equal(results[0], results[2])
+        bits = [r.view(torch.int32) for r in results]          # (the last batch reaches two places nothing was stored in: NaN)
+        assert torch.equal(bits[0], bits[1]) and torch.equal(bits[0], bits[2])
     for gr in graphs:
         gpu.graph_destroy(gr)
 
