@@ -364,16 +364,16 @@ static int attn_shape_check(uint32_t cache_type, size_t page_size, size_t kv_hea
 static AttnPlan attn_plan(int sm_count, size_t n_seqs, size_t M, size_t max_rows, size_t max_len, size_t q_heads, size_t kv_heads, size_t dim, size_t window) {
     AttnPlan p{};
     const size_t group = q_heads / kv_heads, bound = (max_rows < M ? max_rows : M) * group;
-    p.tensor = false;
+    p.tensor = bound > (dim == 256 ? 8 : 16);                // more rows than one warp-level tile: the tcgen05 kernel
     p.mt = bound > 8 && dim <= 128 ? 2 : 1;
-    p.rows = 8 * p.mt;
-    p.block = AR_KEYS;
+    p.rows = p.tensor ? (dim == 256 ? 128 : 256) : 8 * p.mt;
+    p.block = p.tensor && dim != 256 ? 128 : 64;
     const unsigned long long by_seq = (unsigned long long)n_seqs * ((bound + p.rows - 1) / p.rows), by_row = (unsigned long long)M * group / p.rows + n_seqs;
     p.tiles = (long long)(by_seq < by_row ? by_seq : by_row);
     size_t span = max_len;                                   // keys a tile can see at most
     if (window && window + p.rows < span) span = window + p.rows;
     const size_t blocks = span / p.block + 2;
-    const long long slots = (long long)sm_count * (dim == 256 ? 1 : 2), ctas = p.tiles * (long long)kv_heads;
+    const long long slots = (long long)sm_count * (dim == 256 || p.tensor ? 1 : 2), ctas = p.tiles * (long long)kv_heads;
     long long want = ctas >= 4 * slots ? 1 : (2 * slots + ctas - 1) / ctas;
     const long long most = (long long)((blocks + 3) / 4);    // a split of fewer than 4 blocks costs more to start and join than it saves
     if (want > most) want = most;
@@ -466,9 +466,15 @@ extern "C" int ojas_b200_attention(ojas_b200_ctx *ctx, const ojas_b200_kv *kv, c
         a.part_o = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + align256((size_t)p.splits * M * q_heads * sizeof(float2)));
     }
     DeviceGuard guard(ctx->device);
-    cudaError_t e = kv->type == OJAS_B200_BF16 ? launch_rows_dim<true>(ctx, kv, a, p) : launch_rows_dim<false>(ctx, kv, a, p);
-    if (e != cudaSuccess) return ojas_fail(ctx, OJAS_B200_E_CUDA, "launch attn_rows: %s", cudaGetErrorString(e));
-    OJAS_LAUNCH_CHECK(ctx, "attn_rows");
+    cudaError_t e;
+    if (p.tensor) {
+        const int trc = attn_tc_launch(ctx, kv, a, p);
+        if (trc) return trc;
+    } else {
+        e = kv->type == OJAS_B200_BF16 ? launch_rows_dim<true>(ctx, kv, a, p) : launch_rows_dim<false>(ctx, kv, a, p);
+        if (e != cudaSuccess) return ojas_fail(ctx, OJAS_B200_E_CUDA, "launch attn_rows: %s", cudaGetErrorString(e));
+        OJAS_LAUNCH_CHECK(ctx, "attn_rows");
+    }
     if (p.splits > 1) {
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3((unsigned)((M * q_heads + 7) / 8)); cfg.blockDim = dim3(256); cfg.stream = ctx->stream;

@@ -1,0 +1,490 @@
+// Attention for many rows per key head (prompts, chunks of prompts, many query heads to a key head) on the 5th-generation
+// tensor cores: S = Q K^T and O += P V as tcgen05.mma with f32 accumulators in TMEM, tensor-bound (4 dim flops a pair).
+//
+// A CTA takes NQ tiles of 128 rows (rows = token * group + head in group, so a short chunk still fills tiles) of one key head and a
+// range of key blocks.  One warp copies K and V blocks from the pages into a ring (tensor copies, 128-byte swizzle), one thread
+// issues the MMAs, and four warps per tile do the softmax: thread = row = TMEM lane, its scores come out of TMEM into
+// registers, the running maximum and sum stay in registers, and the probabilities go back into TMEM over the scores they came
+// from, where the second product reads them as its A operand.  Q stays in shared memory, O in TMEM.
+//   dim 64, 128: two tiles, keys in blocks of 128; while one tile's softmax runs the tensor cores work for the other tile.
+//   dim 256: one tile (its O takes half of TMEM), keys in blocks of 64, two score buffers: the next block's scores are formed while
+//            the softmax runs.
+// The accumulator is rescaled only when a row's maximum has grown by more than 2^AT_SLACK since it was last fixed (rare after
+// the first blocks): probabilities are kept scaled by 2^AT_SHIFT and stay below f16's limit and above its smallest values.
+//
+// f32 activations enter as two 16-bit terms (TERMS = 2): Q = Qhi + Qlo against the same K, P = Phi + Plo against the same V, twice the
+// MMAs; rows of q are scaled by a power of two so that both terms are in f16's range.  16-bit activations are exact as they
+// are and P is rounded once (relative 2^-12 for f16, 2^-9 for bf16, random over the keys).
+#include "attention.cuh"
+
+namespace {
+
+constexpr float AT_SHIFT = 8.0f, AT_SLACK = 7.0f;
+constexpr int AT_ROWS = 128;
+
+template <int D, int TERMS>
+struct AtShape {
+    static constexpr int NQ = D == 256 ? 1 : 2;                        // row tiles of a CTA
+    static constexpr int KEYS = D == 256 ? 64 : 128;                   // keys of a block
+    static constexpr int STAGE = KEYS * D * 2;                         // one block of K or V
+    static constexpr int Q_TERM = AT_ROWS * D * 2, Q_BYTES = NQ * TERMS * Q_TERM;
+    static constexpr int STAGES_FIT = (232448 - 1024 - 512 - Q_BYTES) / STAGE;
+    static constexpr int STAGES = STAGES_FIT > 6 ? 6 : STAGES_FIT;
+    static constexpr int SMEM = Q_BYTES + STAGES * STAGE + 512 + 1024;
+    static constexpr int SOFT_WARPS = 4 * NQ, THREADS = (SOFT_WARPS + 2) * 32;
+    static constexpr int COL_S = 0, COL_O = 256, O_STEP = 128;         // TMEM columns: scores, accumulators
+    static_assert(STAGES >= 3, "a K and a V block in use and one on the way");
+};
+
+__device__ __forceinline__ void at_ld32(uint32_t taddr, float *v) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+                 "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+                 "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
+                   "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]),
+                   "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]),
+                   "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+                 : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void at_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void at_st16(uint32_t taddr, const uint32_t *v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+                 ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+                   "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]) : "memory");
+}
+__device__ __forceinline__ void at_st32f(uint32_t taddr, const float *v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+                 "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+                 "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+                 ::"r"(taddr), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]), "f"(v[10]),
+                   "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15]), "f"(v[16]), "f"(v[17]), "f"(v[18]), "f"(v[19]), "f"(v[20]), "f"(v[21]),
+                   "f"(v[22]), "f"(v[23]), "f"(v[24]), "f"(v[25]), "f"(v[26]), "f"(v[27]), "f"(v[28]), "f"(v[29]), "f"(v[30]), "f"(v[31]) : "memory");
+}
+__device__ __forceinline__ void at_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// D = A B (accumulate 0) or D += A B; A from shared memory, or from TMEM.
+__device__ __forceinline__ void at_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void at_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// kind::f16: f32 accumulator, M = 128, N = n; `mn`: B is stored with N contiguous (the rows of V).
+__host__ __device__ constexpr uint32_t at_idesc(int n, bool bf, bool mn) {
+    return (1u << 4) | (bf ? (1u << 7) | (1u << 10) : 0u) | (mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(AT_ROWS >> 4) << 24);
+}
+// V as B operand: N (dim) contiguous, 128-byte swizzle; slabs of 64 columns `slab` bytes apart, groups of eight keys 1024 bytes.
+__device__ __forceinline__ uint64_t at_desc_mn(uint32_t smem_addr, uint32_t slab) {
+    return (uint64_t)((smem_addr & 0x3FFFFu) >> 4) | (uint64_t)(slab >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+
+// Rows [r0, r0 + 128) of the sequence (those below r_end) into shared memory as K-major operand tiles (one per term), one row at a
+// time per warp.  Returns this lane's row factor: score -> q . k.
+template <int D, bool BF, int TERMS>
+__device__ __forceinline__ float load_q(const AttnArgs &a, const RowTile &t, int r0, int r_end, int kvh, float sign, unsigned char *tile, int quarter, int lane) {
+    constexpr int V = D / 32;                                              // values per lane: 2, 4 or 8
+    float factor = 1.0f;
+#pragma unroll 4
+    for (int i = 0; i < 32; i++) {
+        const int r = quarter * 32 + i, row = r0 + r;
+        float v[V];
+        const bool live = row < r_end;
+        const long long at = live ? (long long)(t.token0 + row / a.group) * a.q_stride + (long long)(kvh * a.group + row % a.group) * D + lane * V : 0;
+#pragma unroll
+        for (int e = 0; e < V; e += 2) {
+            float2 x = make_float2(0.f, 0.f);
+            if (live) {
+                if (TERMS == 2) x = *reinterpret_cast<const float2 *>(static_cast<const float *>(a.q) + at + e);
+                else x = unpack_half(*reinterpret_cast<const uint32_t *>(static_cast<const uint16_t *>(a.q) + at + e), BF);
+            }
+            v[e] = x.x * sign;
+            v[e + 1] = x.y * sign;
+        }
+        if (TERMS == 2) {
+            float top = 0.0f;
+#pragma unroll
+            for (int e = 0; e < V; e++) top = fmaxf(top, fabsf(v[e]));
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const uint32_t ex = __float_as_uint(top) & 0x7f800000u;        // as in the kernel for few rows
+            const bool scalable = ex > 0x01000000u && ex < 0x7e000000u;
+            const float down = scalable ? __uint_as_float(0x7f000000u - ex) : 1.0f;
+            if (lane == i) factor = scalable ? __uint_as_float(ex) : 1.0f;
+#pragma unroll
+            for (int e = 0; e < V; e++) v[e] *= down;
+        }
+        // element c = lane * V of row r: slab c / 64, 16-byte piece (c % 64) / 8 swizzled by the row
+        const int c = lane * V;
+        const uint32_t off = (uint32_t)((c >> 6) * (AT_ROWS * 128) + r * 128 + ((((c & 63) >> 3) ^ (r & 7)) << 4) + (c & 7) * 2);
+        uint32_t hi[V / 2], lo[V / 2];
+#pragma unroll
+        for (int e = 0; e < V / 2; e++) {
+            hi[e] = pack_half(v[2 * e], v[2 * e + 1], BF);
+            const float2 h = unpack_half(hi[e], BF);
+            lo[e] = pack_half(v[2 * e] - h.x, v[2 * e + 1] - h.y, BF);
+        }
+#pragma unroll
+        for (int e = 0; e < V / 2; e++) {
+            *reinterpret_cast<uint32_t *>(tile + off + 4 * e) = hi[e];
+            if (TERMS == 2) *reinterpret_cast<uint32_t *>(tile + AT_ROWS * D * 2 + off + 4 * e) = lo[e];
+        }
+    }
+    return factor;
+}
+
+template <int D, bool BF, int TERMS>
+__global__ void __launch_bounds__(AtShape<D, TERMS>::THREADS, 1) attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k,
+                                                                                  const __grid_constant__ CUtensorMap map_v, const AttnArgs a, int box_rows) {
+    using S = AtShape<D, TERMS>;
+    constexpr int NQ = S::NQ, KEYS = S::KEYS, STAGES = S::STAGES, STAGE = S::STAGE;
+    extern __shared__ unsigned char at_raw[];
+    unsigned char *smem = reinterpret_cast<unsigned char *>(((uintptr_t)at_raw + 1023) & ~(uintptr_t)1023);
+    unsigned char *ring = smem + S::Q_BYTES;
+    uint64_t *bars = reinterpret_cast<uint64_t *>(ring + STAGES * STAGE);
+    uint64_t *kv_full = bars, *kv_empty = bars + 8, *s_full = bars + 16, *p_full = bars + 18, *o_done = bars + 20, *q_full = bars + 22, *raw = bars + 24;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 26);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kvh = blockIdx.y, split = blockIdx.z;
+    unsigned *status = a.batch.status;
+    constexpr unsigned CODE = OJAS_ST_ATTN_WAIT;
+
+    grid_launch_dependents();
+    grid_dependency_wait();
+    // long tiles first: the last rows of a sequence see the most keys
+    RowTile t;
+    if (!find_tile(a, gridDim.x - 1 - blockIdx.x, NQ * AT_ROWS, lane, t)) return;
+    const int rows = min(NQ * AT_ROWS, t.n_rows - t.row0);
+    int lo, hi;
+    key_range(a, t, t.row0, t.row0 + rows, lo, hi);
+    const int all0 = lo / KEYS, all1 = hi > lo ? (hi + KEYS - 1) / KEYS : all0;
+    const bool alone = a.splits == 1 || all1 - all0 <= a.split_blocks;
+    if (alone && split > 0) return;
+    const int blk0 = min(all1, all0 + split * a.split_blocks), blk1 = split == a.splits - 1 ? all1 : min(all1, blk0 + a.split_blocks);
+    // each tile's own part of the blocks (a tile without rows: none)
+    int first[NQ], last[NQ];
+#pragma unroll
+    for (int u = 0; u < NQ; u++) {
+        first[u] = last[u] = blk0;
+        const int r0 = t.row0 + u * AT_ROWS, r1 = min(r0 + AT_ROWS, t.n_rows);
+        if (r1 > r0) {
+            int l, h;
+            key_range(a, t, r0, r1, l, h);
+            if (h > l) { first[u] = min(blk1, max(blk0, l / KEYS)); last[u] = max(first[u], min(blk1, (h + KEYS - 1) / KEYS)); }
+        }
+    }
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; s++) { mbar_init(&kv_full[s], 1); mbar_init(&kv_empty[s], 1); }
+        for (int u = 0; u < 2; u++) { mbar_init(&s_full[u], 1); mbar_init(&p_full[u], 4); mbar_init(&o_done[u], 1); mbar_init(&q_full[u], 4); }
+        mbar_init(raw, 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&map_k) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&map_v) : "memory");
+    }
+    if (warp == S::SOFT_WARPS) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp < S::SOFT_WARPS) {
+        // ---------------- softmax of tile u: thread = row
+        const int u = warp >> 2, quarter = warp & 3;
+        const int r0 = t.row0 + u * AT_ROWS, row = r0 + quarter * 32 + lane;
+        const bool live = row < t.n_rows;
+        unsigned char *q_tile = smem + u * TERMS * S::Q_TERM;
+        float factor = load_q<D, BF, TERMS>(a, t, r0, t.n_rows, kvh, a.scale_log2 < 0.0f ? -1.0f : 1.0f, q_tile, quarter, lane);
+        factor = fminf(fmaxf(factor * fabsf(a.scale_log2), 1e-37f), 3e38f);  // a masked score (-inf) has to stay -inf when multiplied
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_full[u]);
+        int see_lo = 0, see_hi = 0;
+        if (live) row_range(a, t, row, see_lo, see_hi);
+        const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
+        const uint32_t o_col = lane_base + S::COL_O + u * S::O_STEP;
+        float m = -INFINITY, l = 0.0f;
+        bool ok = true;
+        for (int blk = first[u], n = 0; blk < last[u]; blk++, n++) {
+            const int sb = NQ == 2 ? u : n & 1;
+            const uint32_t s_col = lane_base + S::COL_S + sb * 128;
+            if (!mbar_wait_warp(&s_full[sb], NQ == 2 ? (uint32_t)n & 1u : (uint32_t)(n >> 1) & 1u, abort_flag, status, CODE)) { ok = false; break; }
+            tc_fence_after();
+            float x[KEYS];
+#pragma unroll
+            for (int c = 0; c < KEYS; c += 32) at_ld32(s_col + c, x + c);
+            at_wait_ld();
+            const int key0 = blk * KEYS;
+            if (__any_sync(0xffffffffu, key0 < see_lo || key0 + KEYS > see_hi)) {
+                const unsigned span = (unsigned)max(0, see_hi - see_lo);
+#pragma unroll
+                for (int c = 0; c < KEYS; c++)
+                    if ((unsigned)(key0 + c - see_lo) >= span) x[c] = -INFINITY;
+            }
+            float top = x[0];
+#pragma unroll
+            for (int c = 1; c < KEYS; c++) top = fmaxf(top, x[c]);
+            top *= factor;
+            const bool grow = top > m + AT_SLACK;
+            if (__any_sync(0xffffffffu, grow)) {
+                const float mn = grow ? top : m;
+                const float f = mn == m ? 1.0f : exp2_fast(m - mn);
+                m = mn;
+                l *= f;
+                if (n > 0) {
+                    // the product of the block before has to be in O: with one score buffer its completion came before these
+                    // scores', with two it has a barrier of its own
+                    if (NQ == 1) {
+                        if (!mbar_wait_warp(&o_done[0], (uint32_t)(n - 1) & 1u, abort_flag, status, CODE)) { ok = false; break; }
+                        tc_fence_after();
+                    }
+#pragma unroll 1
+                    for (int c = 0; c < D; c += 32) {
+                        float o[32];
+                        at_ld32(o_col + c, o);
+                        at_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; i++) o[i] *= f;
+                        at_st32f(o_col + c, o);
+                    }
+                }
+            }
+            const float off = m == -INFINITY ? 0.0f : m - AT_SHIFT;
+            float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < KEYS; c += 32) {
+                uint32_t hi16[16], lo16[16];
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const float p0 = exp2_fast(fmaf(x[c + 2 * i], factor, -off)), p1 = exp2_fast(fmaf(x[c + 2 * i + 1], factor, -off));
+                    part[i & 3] += p0 + p1;
+                    hi16[i] = pack_half(p0, p1, BF);
+                    if (TERMS == 2) {
+                        const float2 h = unpack_half(hi16[i], BF);
+                        lo16[i] = pack_half(p0 - h.x, p1 - h.y, BF);
+                    }
+                }
+                at_st16(s_col + c / 2, hi16);
+                if (TERMS == 2) at_st16(s_col + KEYS / 2 + c / 2, lo16);
+            }
+            l += (part[0] + part[1]) + (part[2] + part[3]);
+            at_wait_st();
+            // With two score buffers the scores run a block ahead: passing these probabilities on only when the product before has
+            // ended keeps every waiter within one phase of its barrier (a parity cannot tell a phase from the one two before).
+            if (NQ == 1 && n > 0 && !mbar_wait_warp(&o_done[0], (uint32_t)(n - 1) & 1u, abort_flag, status, CODE)) { ok = false; break; }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[u]);
+        }
+        // ---------------- the tile's rows: O / l to out, or O and (m, l) to the split's place
+        const int blocks = last[u] - first[u];
+        if (ok && blocks > 0) {
+            ok = mbar_wait_warp(&o_done[u], NQ == 2 ? 0u : (uint32_t)(blocks - 1) & 1u, abort_flag, status, CODE);
+            tc_fence_after();
+        }
+        if (ok) {
+            const long long token = live ? t.token0 + row / a.group : 0;
+            const int head = kvh * a.group + row % a.group;
+            const long long slot = ((long long)split * a.batch.M + token) * a.q_heads + head;
+            const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+            if (live && !alone) a.part_ml[slot] = make_float2(m, l);
+            if (live && alone && a.part_ml) a.part_ml[token * a.q_heads + head] = make_float2(0.0f, -1.0f);
+            if (alone || blk1 > blk0) {
+#pragma unroll 1
+                for (int c = 0; c < D; c += 32) {
+                    float o[32];
+                    if (blocks > 0) {
+                        at_ld32(o_col + c, o);
+                        at_wait_ld();
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; i++) o[i] = 0.0f;
+                    }
+                    __syncwarp();
+                    const long long at = alone ? token * a.out_stride + (long long)head * D + c : slot * D + c;
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) {
+                        const float4 v = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                        if (!live) { }
+                        else if (alone) store_elem4(a.out, a.act_type, at + i, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+                        else *reinterpret_cast<float4 *>(a.part_o + at + i) = v;
+                    }
+                }
+            }
+        }
+    } else if (warp == S::SOFT_WARPS) {
+        // ---------------- MMA issue (one thread); ring order: see the loader
+        if (lane == 0) {
+            constexpr uint32_t ID_S = at_idesc(KEYS, BF, false), ID_O = at_idesc(D, BF, true);
+            bool ok = true;
+            int s = 0;
+            uint32_t phase = 0;
+            auto next = [&]() { if (++s == STAGES) { s = 0; phase ^= 1u; } };
+            auto wait = [&](uint64_t *bar, uint32_t parity) { ok = ok && mbar_wait_spin(bar, parity, abort_flag, status, CODE); };
+            auto scores = [&](int u, int buf, int stage) {
+                const uint64_t kd = umma_desc(smem_u32(ring + stage * STAGE));
+#pragma unroll
+                for (int term = 0; term < TERMS; term++) {
+                    const uint64_t qd = umma_desc(smem_u32(smem + (u * TERMS + term) * S::Q_TERM));
+#pragma unroll
+                    for (int k = 0; k < D / 16; k++)     // 16 of dim: 32 bytes of a row, four per slab
+                        at_mma_ss(tmem + S::COL_S + buf * 128, qd + (k >> 2) * (AT_ROWS * 128 / 16) + (k & 3) * 2, kd + (k >> 2) * (KEYS * 128 / 16) + (k & 3) * 2, ID_S,
+                                  term + k > 0);
+                }
+                umma_commit(&s_full[buf]);
+            };
+            auto values = [&](int u, int buf, int stage, bool begin) {
+                const uint64_t vd = at_desc_mn(smem_u32(ring + stage * STAGE), KEYS * 128);
+#pragma unroll
+                for (int term = 0; term < TERMS; term++)
+#pragma unroll
+                    for (int k = 0; k < KEYS / 16; k++)  // 16 keys: 8 columns of packed P, 2048 bytes of V
+                        at_mma_ts(tmem + S::COL_O + u * S::O_STEP, tmem + S::COL_S + buf * 128 + term * (KEYS / 2) + k * 8, vd + k * (2048 / 16), ID_O, !begin || term + k > 0);
+            };
+            for (int u = 0; u < NQ; u++)
+                if (last[u] > first[u]) wait(&q_full[u], 0);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            if (NQ == 2) {
+                int v_stage = 0, n[2] = {0, 0};
+                for (int i = blk0; ok && i <= blk1; i++) {
+                    // block i's K is at the ring's head, block i - 1's V one behind it: (K0) (V0 K1) (V1 K2) ... (Vlast)
+                    if (i > blk0) { wait(&kv_full[s], phase); v_stage = s; next(); }
+                    const int k_stage = s;
+                    if (i < blk1) { wait(&kv_full[s], phase); next(); }
+                    if (!ok) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int u = 0; u < NQ; u++) {
+                        if (i - 1 >= first[u] && i - 1 < last[u]) {
+                            wait(&p_full[u], (uint32_t)n[u] & 1u);
+                            if (!ok) break;
+                            tc_fence_after();
+                            values(u, u, v_stage, n[u] == 0);
+                            n[u]++;
+                            if (i == last[u]) umma_commit(&o_done[u]);
+                        }
+                        if (u == NQ - 1 && i > blk0) umma_commit(&kv_empty[v_stage]);
+                        if (i >= first[u] && i < last[u]) scores(u, u, k_stage);
+                        if (u == NQ - 1 && i < blk1) umma_commit(&kv_empty[k_stage]);
+                    }
+                }
+            } else {
+                for (int i = blk0; ok && i <= blk1; i++) {
+                    // (K0) (K1 V0) (K2 V1) ... (Vlast)
+                    if (i < blk1) {
+                        wait(&kv_full[s], phase);
+                        if (!ok) break;
+                        tc_fence_after();
+                        scores(0, (i - blk0) & 1, s);
+                        umma_commit(&kv_empty[s]);
+                        next();
+                    }
+                    if (i > blk0) {
+                        const int n = i - 1 - blk0;
+                        wait(&kv_full[s], phase);
+                        wait(&p_full[0], (uint32_t)n & 1u);
+                        if (!ok) break;
+                        tc_fence_after();
+                        values(0, n & 1, s, n == 0);
+                        umma_commit(&o_done[0]);
+                        umma_commit(&kv_empty[s]);
+                        next();
+                    }
+                }
+            }
+        }
+    } else {
+        // ---------------- loader: lane = one box (64 values x box_rows tokens).  NQ 2: K0 V0 K1 V1 ...; NQ 1: K0 K1 V0 K2 V1 ...
+        const int per_slab = KEYS / box_rows, boxes = per_slab * (D / 64);
+        int s = 0;
+        uint32_t phase = 1, raw_phase = 0;
+        const int n = blk1 - blk0;
+        bool ok = true;
+        for (int i = 0; ok && i < 2 * n; i++) {
+            // the i-th block of the ring: which block, K or V
+            const bool is_v = NQ == 2 ? (i & 1) : i == 2 * n - 1 || (i >= 2 && (i & 1) == 0);
+            const int b = NQ == 2 ? i >> 1 : is_v ? (i == 2 * n - 1 ? n - 1 : i / 2 - 1) : (i + 1) / 2;
+            const int blk = blk0 + b;
+            if (!mbar_wait_warp(&kv_empty[s], phase, abort_flag, status, CODE)) break;
+            unsigned char *to = ring + s * STAGE;
+            const int part = lane % per_slab, slab = lane / per_slab, key = blk * KEYS + part * box_rows;
+            const bool want = lane < boxes && key < hi && key + box_rows > lo;
+            int page = 0;
+            if (want) {
+                page = __ldg(a.batch.table + (long long)t.seq * a.batch.table_stride + key / a.batch.page_size);
+                if (page < 0 || page >= a.batch.pages) { atomicOr(status, OJAS_ST_BATCH); page = a.batch.pages; }      // reads as zeros
+            }
+            const int copies = __popc(__ballot_sync(0xffffffffu, want));
+            // the values of keys that are not read must be zeros (0 * NaN is NaN): such a block lands on a barrier of the loader's own
+            // and is passed on after they are
+            const bool edge = is_v && (blk * KEYS < lo || (blk + 1) * KEYS > hi);
+            uint64_t *bar = edge ? raw : &kv_full[s];
+            if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(copies * box_rows * 128));
+            __syncwarp();
+            if (want)
+                tma_load_4d(to + slab * (KEYS * 128) + part * box_rows * 128, is_v ? &map_v : &map_k, slab * 64, key % a.batch.page_size, kvh, page, bar);
+            if (edge) {
+                ok = mbar_wait_warp(raw, raw_phase, abort_flag, status, CODE);
+                raw_phase ^= 1u;
+                for (int e = lane; e < KEYS * (D / 8); e += 32) {          // 16-byte pieces; a row's pieces may be zeroed in any order
+                    const int r = e / (D / 8), c = e % (D / 8);
+                    if (blk * KEYS + r < lo || blk * KEYS + r >= hi) *reinterpret_cast<uint4 *>(to + (c >> 3) * (KEYS * 128) + r * 128 + (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&kv_full[s]);
+            }
+            if (++s == STAGES) { s = 0; phase ^= 1u; }
+        }
+    }
+
+    // ---------------- teardown: every role arrives here, also after an abort (copies and MMAs in flight then get a bounded time)
+    if (*abort_flag) {
+        const long long t0 = clock64();
+        while (clock64() - t0 < 2000000LL) { }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == S::SOFT_WARPS) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+template <int D, bool BF, int TERMS>
+cudaError_t launch_tiles(const ojas_b200_ctx *ctx, const ojas_b200_kv *kv, const AttnArgs &a, const AttnPlan &p) {
+    using S = AtShape<D, TERMS>;
+    cudaError_t e = cudaFuncSetAttribute(attn_tiles_kernel<D, BF, TERMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)p.tiles, (unsigned)kv->heads, (unsigned)p.splits);
+    cfg.blockDim = dim3(S::THREADS);
+    cfg.dynamicSmemBytes = S::SMEM;
+    cfg.stream = ctx->stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = ctx->pdl ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, attn_tiles_kernel<D, BF, TERMS>, kv->map_k, kv->map_v, a, kv->box_rows);
+}
+template <bool BF, int TERMS>
+cudaError_t launch_tiles_dim(const ojas_b200_ctx *ctx, const ojas_b200_kv *kv, const AttnArgs &a, const AttnPlan &p) {
+    return kv->dim == 64 ? launch_tiles<64, BF, TERMS>(ctx, kv, a, p) : kv->dim == 128 ? launch_tiles<128, BF, TERMS>(ctx, kv, a, p) : launch_tiles<256, BF, TERMS>(ctx, kv, a, p);
+}
+
+}  // namespace
+
+int attn_tc_launch(ojas_b200_ctx *ctx, const ojas_b200_kv *kv, const AttnArgs &a, const AttnPlan &p) {
+    const bool bf = kv->type == OJAS_B200_BF16, two = a.act_type == OJAS_B200_F32;
+    const cudaError_t e = bf ? (two ? launch_tiles_dim<true, 2>(ctx, kv, a, p) : launch_tiles_dim<true, 1>(ctx, kv, a, p))
+                             : (two ? launch_tiles_dim<false, 2>(ctx, kv, a, p) : launch_tiles_dim<false, 1>(ctx, kv, a, p));
+    if (e != cudaSuccess) return ojas_fail(ctx, OJAS_B200_E_CUDA, "launch attn_tiles: %s", cudaGetErrorString(e));
+    OJAS_LAUNCH_CHECK(ctx, "attn_tiles");
+    return 0;
+}
