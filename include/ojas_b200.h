@@ -358,8 +358,8 @@ OJAS_B200_API int ojas_b200_kv_append_check(size_t kv_heads, size_t dim, size_t 
  * Behind a sequence's end the cache may hold anything; a key that only some rows of a call see must be finite for the
  * others.  workspace: caller-owned scratch of ojas_b200_attention_workspace_bytes (0: may be null), 256-byte aligned, not
  * shared by calls that may run at the same time. */
-OJAS_B200_API size_t ojas_b200_attention_workspace_bytes(ojas_b200_ctx *ctx, const ojas_b200_kv *kv, const ojas_b200_seqs *seqs, size_t M,
-                                                         size_t q_heads, long long window);
+OJAS_B200_API size_t ojas_b200_attention_workspace_bytes(ojas_b200_ctx *ctx, const ojas_b200_kv *kv, const ojas_b200_seqs *seqs,
+                                                         uint32_t act_type, size_t M, size_t q_heads, long long window);
 OJAS_B200_API int ojas_b200_attention(ojas_b200_ctx *ctx, const ojas_b200_kv *kv, const ojas_b200_seqs *seqs, uint32_t act_type, const void *q,
                                       size_t q_stride, size_t q_heads, float scale, int causal, long long window, void *out, size_t out_stride,
                                       size_t M, void *workspace, size_t workspace_bytes);

@@ -361,12 +361,12 @@ static int attn_shape_check(uint32_t cache_type, size_t page_size, size_t kv_hea
 }
 
 // Which kernel, and how far the keys are split so that few rows still use every SM.
-static AttnPlan attn_plan(int sm_count, size_t n_seqs, size_t M, size_t max_rows, size_t max_len, size_t q_heads, size_t kv_heads, size_t dim, size_t window) {
+static AttnPlan attn_plan(int sm_count, size_t n_seqs, size_t M, size_t max_rows, size_t max_len, size_t q_heads, size_t kv_heads, size_t dim, size_t window, bool f32) {
     AttnPlan p{};
     const size_t group = q_heads / kv_heads, bound = (max_rows < M ? max_rows : M) * group;
     p.tensor = bound > (dim == 256 ? 8 : 16);                // more rows than one warp-level tile: the tcgen05 kernel
     p.mt = bound > 8 && dim <= 128 ? 2 : 1;
-    p.rows = p.tensor ? (dim == 256 ? 128 : 256) : 8 * p.mt;
+    p.rows = p.tensor ? (dim == 256 || f32 ? 128 : 256) : 8 * p.mt;
     p.block = p.tensor && dim != 256 ? 128 : 64;
     const unsigned long long by_seq = (unsigned long long)n_seqs * ((bound + p.rows - 1) / p.rows), by_row = (unsigned long long)M * group / p.rows + n_seqs;
     p.tiles = (long long)(by_seq < by_row ? by_seq : by_row);
@@ -374,7 +374,7 @@ static AttnPlan attn_plan(int sm_count, size_t n_seqs, size_t M, size_t max_rows
     if (window && window + p.rows < span) span = window + p.rows;
     const size_t blocks = span / p.block + 2;
     const long long slots = (long long)sm_count * (dim == 256 || p.tensor ? 1 : 2), ctas = p.tiles * (long long)kv_heads;
-    long long want = ctas >= 4 * slots ? 1 : (2 * slots + ctas - 1) / ctas;
+    long long want = p.tensor ? slots / ctas : ctas >= 4 * slots ? 1 : (2 * slots + ctas - 1) / ctas;
     const long long most = (long long)((blocks + 3) / 4);    // a split of fewer than 4 blocks costs more to start and join than it saves
     if (want > most) want = most;
     if (want > 1024) want = 1024;
@@ -407,10 +407,11 @@ extern "C" int ojas_b200_attention_check(uint32_t cache_type, size_t page_size, 
     return 0;
 }
 
-extern "C" size_t ojas_b200_attention_workspace_bytes(ojas_b200_ctx *ctx, const ojas_b200_kv *kv, const ojas_b200_seqs *seqs, size_t M, size_t q_heads, long long window) {
+extern "C" size_t ojas_b200_attention_workspace_bytes(ojas_b200_ctx *ctx, const ojas_b200_kv *kv, const ojas_b200_seqs *seqs, uint32_t act_type, size_t M, size_t q_heads,
+                                                      long long window) {
     if (!ctx || !kv || !seqs || window < 0 || M == 0 || seqs->n_seqs == 0) return 0;
-    if (attn_shape_check(kv->type, kv->page_size, kv->heads, kv->dim, kv->type, q_heads, M, seqs->max_rows, seqs->max_len, nullptr, 0)) return 0;
-    return attn_plan(ctx->sm_count, seqs->n_seqs, M, seqs->max_rows, seqs->max_len, q_heads, kv->heads, kv->dim, (size_t)window).workspace;
+    if (attn_shape_check(kv->type, kv->page_size, kv->heads, kv->dim, act_type, q_heads, M, seqs->max_rows, seqs->max_len, nullptr, 0)) return 0;
+    return attn_plan(ctx->sm_count, seqs->n_seqs, M, seqs->max_rows, seqs->max_len, q_heads, kv->heads, kv->dim, (size_t)window, act_type == OJAS_B200_F32).workspace;
 }
 
 template <int D, bool BF, int MT>
@@ -446,7 +447,7 @@ extern "C" int ojas_b200_attention(ojas_b200_ctx *ctx, const ojas_b200_kv *kv, c
     const int rc = ojas_b200_attention_check(kv->type, kv->page_size, kv->heads, kv->dim, act_type, q_heads, q, q_stride, out, out_stride, scale, causal, window, seqs, M, why, sizeof why);
     if (rc) return ojas_fail(ctx, rc, "%s", why);
     if (M == 0 || seqs->n_seqs == 0) return 0;
-    const AttnPlan p = attn_plan(ctx->sm_count, seqs->n_seqs, M, seqs->max_rows, seqs->max_len, q_heads, kv->heads, kv->dim, (size_t)window);
+    const AttnPlan p = attn_plan(ctx->sm_count, seqs->n_seqs, M, seqs->max_rows, seqs->max_len, q_heads, kv->heads, kv->dim, (size_t)window, act_type == OJAS_B200_F32);
     if (p.workspace) {
         if (!workspace || workspace_bytes < p.workspace) return ojas_fail(ctx, OJAS_B200_E_ARG, "attention: workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : 0, p.workspace);
         if ((uintptr_t)workspace % 256) return ojas_fail(ctx, OJAS_B200_E_ARG, "attention: the workspace must start on 256 bytes");

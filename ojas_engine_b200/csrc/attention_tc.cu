@@ -6,15 +6,20 @@
 // issues the MMAs, and four warps per tile do the softmax: thread = row = TMEM lane, its scores come out of TMEM into
 // registers, the running maximum and sum stay in registers, and the probabilities go back into TMEM over the scores they came
 // from, where the second product reads them as its A operand.  Q stays in shared memory, O in TMEM.
-//   dim 64, 128: two tiles, keys in blocks of 128; while one tile's softmax runs the tensor cores work for the other tile.
-//   dim 256: one tile (its O takes half of TMEM), keys in blocks of 64, two score buffers: the next block's scores are formed while
-//            the softmax runs.
+//   NQ = 2 (dim 64 and 128, 16-bit activations): while one tile's softmax runs the tensor cores work for the other tile.
+//   NQ = 1 (dim 256, whose O takes half of TMEM, and f32 activations): two score buffers; the next block's scores are formed
+//          while the softmax runs.
 // The accumulator is rescaled only when a row's maximum has grown by more than 2^AT_SLACK since it was last fixed (rare after
 // the first blocks): probabilities are kept scaled by 2^AT_SHIFT and stay below f16's limit and above its smallest values.
 //
 // f32 activations enter as two 16-bit terms (TERMS = 2): Q = Qhi + Qlo against the same K, P = Phi + Plo against the same V, twice the
 // MMAs; rows of q are scaled by a power of two so that both terms are in f16's range.  16-bit activations are exact as they
 // are and P is rounded once (relative 2^-12 for f16, 2^-9 for bf16, random over the keys).
+//
+// The tensor cores cut what they add to an accumulator: every instruction takes up to 2^-23 off |O|, always towards zero, and
+// thousands of them over a long context took 1.2e-5 off an f32 result (12 000 keys).  With f32 activations O is therefore added,
+// in rounded f32, to sums of its own every 512 keys: in TMEM, or for dim 256, which leaves no room there, in the row's place
+// in memory.
 #include "attention.cuh"
 
 namespace {
@@ -24,7 +29,7 @@ constexpr int AT_ROWS = 128;
 
 template <int D, int TERMS>
 struct AtShape {
-    static constexpr int NQ = D == 256 ? 1 : 2;                        // row tiles of a CTA
+    static constexpr int NQ = D == 256 || TERMS == 2 ? 1 : 2;          // row tiles of a CTA
     static constexpr int KEYS = D == 256 ? 64 : 128;                   // keys of a block
     static constexpr int STAGE = KEYS * D * 2;                         // one block of K or V
     static constexpr int Q_TERM = AT_ROWS * D * 2, Q_BYTES = NQ * TERMS * Q_TERM;
@@ -33,6 +38,8 @@ struct AtShape {
     static constexpr int SMEM = Q_BYTES + STAGES * STAGE + 512 + 1024;
     static constexpr int SOFT_WARPS = 4 * NQ, THREADS = (SOFT_WARPS + 2) * 32;
     static constexpr int COL_S = 0, COL_O = 256, O_STEP = 128;         // TMEM columns: scores, accumulators
+    static constexpr int COL_SUM = 384;                                // TERMS 2, dim <= 128: the sums of earlier blocks
+    static constexpr int FLUSH = TERMS == 2 ? 512 / KEYS : 1 << 30;    // blocks after which O is added to those sums
     static_assert(STAGES >= 3, "a K and a V block in use and one on the way");
 };
 
@@ -80,56 +87,87 @@ __device__ __forceinline__ uint64_t at_desc_mn(uint32_t smem_addr, uint32_t slab
     return (uint64_t)((smem_addr & 0x3FFFFu) >> 4) | (uint64_t)(slab >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
 
-// Rows [r0, r0 + 128) of the sequence (those below r_end) into shared memory as K-major operand tiles (one per term), one row at a
-// time per warp.  Returns this lane's row factor: score -> q . k.
-template <int D, bool BF, int TERMS>
-__device__ __forceinline__ float load_q(const AttnArgs &a, const RowTile &t, int r0, int r_end, int kvh, float sign, unsigned char *tile, int quarter, int lane) {
-    constexpr int V = D / 32;                                              // values per lane: 2, 4 or 8
-    float factor = 1.0f;
-#pragma unroll 4
-    for (int i = 0; i < 32; i++) {
-        const int r = quarter * 32 + i, row = r0 + r;
-        float v[V];
-        const bool live = row < r_end;
-        const long long at = live ? (long long)(t.token0 + row / a.group) * a.q_stride + (long long)(kvh * a.group + row % a.group) * D + lane * V : 0;
+// sums = sums * by + O (first time: sums = O) for this thread's row, and O may be overwritten.
+template <int D>
+__device__ __forceinline__ void add_to_sums(uint32_t o_col, uint32_t sum_col, float *sums, bool live, bool more, float by) {
+#pragma unroll 1
+    for (int c = 0; c < D; c += 32) {
+        float o[32];
+        at_ld32(o_col + c, o);
+        if (D <= 128) {
+            if (more) {
+                float e[32];
+                at_ld32(sum_col + c, e);
+                at_wait_ld();
 #pragma unroll
-        for (int e = 0; e < V; e += 2) {
-            float2 x = make_float2(0.f, 0.f);
-            if (live) {
-                if (TERMS == 2) x = *reinterpret_cast<const float2 *>(static_cast<const float *>(a.q) + at + e);
-                else x = unpack_half(*reinterpret_cast<const uint32_t *>(static_cast<const uint16_t *>(a.q) + at + e), BF);
+                for (int i = 0; i < 32; i++) o[i] = fmaf(e[i], by, o[i]);
             }
-            v[e] = x.x * sign;
-            v[e + 1] = x.y * sign;
+            at_wait_ld();
+            at_st32f(sum_col + c, o);
+        } else {
+            at_wait_ld();
+            if (live) {
+#pragma unroll
+                for (int i = 0; i < 32; i += 4) {
+                    float4 v = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                    if (more) {
+                        const float4 e = *reinterpret_cast<const float4 *>(sums + c + i);
+                        v = make_float4(fmaf(e.x, by, v.x), fmaf(e.y, by, v.y), fmaf(e.z, by, v.z), fmaf(e.w, by, v.w));
+                    }
+                    *reinterpret_cast<float4 *>(sums + c + i) = v;
+                }
+            }
+            __syncwarp();
         }
-        if (TERMS == 2) {
-            float top = 0.0f;
-#pragma unroll
-            for (int e = 0; e < V; e++) top = fmaxf(top, fabsf(v[e]));
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            const uint32_t ex = __float_as_uint(top) & 0x7f800000u;        // as in the kernel for few rows
-            const bool scalable = ex > 0x01000000u && ex < 0x7e000000u;
-            const float down = scalable ? __uint_as_float(0x7f000000u - ex) : 1.0f;
-            if (lane == i) factor = scalable ? __uint_as_float(ex) : 1.0f;
-#pragma unroll
-            for (int e = 0; e < V; e++) v[e] *= down;
+    }
+}
+
+// This thread's row of q (nothing: zeros) into shared memory as K-major operand tiles, one per term.  Returns the row's factor:
+// score -> q . k.
+template <int D, bool BF, int TERMS>
+__device__ __forceinline__ float load_q(const void *q, long long at, bool live, float sign, unsigned char *tile, int r) {
+    float factor = 1.0f, by = sign;
+    if (TERMS == 2) {
+        const float *src = static_cast<const float *>(q) + at;
+        float top = 0.0f;
+        if (live) {
+#pragma unroll 16
+            for (int c = 0; c < D; c += 4) {
+                const float4 v = *reinterpret_cast<const float4 *>(src + c);
+                top = fmaxf(top, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
+            }
         }
-        // element c = lane * V of row r: slab c / 64, 16-byte piece (c % 64) / 8 swizzled by the row
-        const int c = lane * V;
-        const uint32_t off = (uint32_t)((c >> 6) * (AT_ROWS * 128) + r * 128 + ((((c & 63) >> 3) ^ (r & 7)) << 4) + (c & 7) * 2);
-        uint32_t hi[V / 2], lo[V / 2];
-#pragma unroll
-        for (int e = 0; e < V / 2; e++) {
-            hi[e] = pack_half(v[2 * e], v[2 * e + 1], BF);
-            const float2 h = unpack_half(hi[e], BF);
-            lo[e] = pack_half(v[2 * e] - h.x, v[2 * e + 1] - h.y, BF);
+        const uint32_t ex = __float_as_uint(top) & 0x7f800000u;            // as in the kernel for few rows
+        if (ex > 0x01000000u && ex < 0x7e000000u) {
+            factor = __uint_as_float(ex);
+            by = sign * __uint_as_float(0x7f000000u - ex);
         }
+    }
+#pragma unroll 8
+    for (int c = 0; c < D; c += 8) {
+        // elements c .. c + 7 of row r: slab c / 64, 16-byte piece (c % 64) / 8 swizzled by the row
+        unsigned char *to = tile + (c >> 6) * (AT_ROWS * 128) + r * 128 + ((((c & 63) >> 3) ^ (r & 7)) << 4);
+        uint32_t hi[4] = {0u, 0u, 0u, 0u}, lo[4] = {0u, 0u, 0u, 0u};
+        if (live) {
+            if (TERMS == 2) {
+                const float4 x = *reinterpret_cast<const float4 *>(static_cast<const float *>(q) + at + c);
+                const float4 y = *reinterpret_cast<const float4 *>(static_cast<const float *>(q) + at + c + 4);
+                const float v[8] = {x.x * by, x.y * by, x.z * by, x.w * by, y.x * by, y.y * by, y.z * by, y.w * by};
 #pragma unroll
-        for (int e = 0; e < V / 2; e++) {
-            *reinterpret_cast<uint32_t *>(tile + off + 4 * e) = hi[e];
-            if (TERMS == 2) *reinterpret_cast<uint32_t *>(tile + AT_ROWS * D * 2 + off + 4 * e) = lo[e];
+                for (int e = 0; e < 4; e++) {
+                    hi[e] = pack_half(v[2 * e], v[2 * e + 1], BF);
+                    const float2 h = unpack_half(hi[e], BF);
+                    lo[e] = pack_half(v[2 * e] - h.x, v[2 * e + 1] - h.y, BF);
+                }
+            } else {
+                const uint16_t *src = static_cast<const uint16_t *>(q) + at + c;   // rows start on 8 bytes
+                const uint2 x = *reinterpret_cast<const uint2 *>(src), y = *reinterpret_cast<const uint2 *>(src + 4);
+                const uint32_t flip = sign < 0.0f ? 0x80008000u : 0u;
+                hi[0] = x.x ^ flip; hi[1] = x.y ^ flip; hi[2] = y.x ^ flip; hi[3] = y.y ^ flip;
+            }
         }
+        *reinterpret_cast<uint4 *>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        if (TERMS == 2) *reinterpret_cast<uint4 *>(to + AT_ROWS * D * 2) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
     return factor;
 }
@@ -199,7 +237,9 @@ __global__ void __launch_bounds__(AtShape<D, TERMS>::THREADS, 1) attn_tiles_kern
         const int r0 = t.row0 + u * AT_ROWS, row = r0 + quarter * 32 + lane;
         const bool live = row < t.n_rows;
         unsigned char *q_tile = smem + u * TERMS * S::Q_TERM;
-        float factor = load_q<D, BF, TERMS>(a, t, r0, t.n_rows, kvh, a.scale_log2 < 0.0f ? -1.0f : 1.0f, q_tile, quarter, lane);
+        const long long token = live ? t.token0 + row / a.group : 0;
+        const int head = kvh * a.group + (live ? row % a.group : 0);
+        float factor = load_q<D, BF, TERMS>(a.q, token * a.q_stride + (long long)head * D, live, a.scale_log2 < 0.0f ? -1.0f : 1.0f, q_tile, quarter * 32 + lane);
         factor = fminf(fmaxf(factor * fabsf(a.scale_log2), 1e-37f), 3e38f);  // a masked score (-inf) has to stay -inf when multiplied
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
@@ -208,7 +248,10 @@ __global__ void __launch_bounds__(AtShape<D, TERMS>::THREADS, 1) attn_tiles_kern
         if (live) row_range(a, t, row, see_lo, see_hi);
         const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
         const uint32_t o_col = lane_base + S::COL_O + u * S::O_STEP;
-        float m = -INFINITY, l = 0.0f;
+        const long long slot = ((long long)split * a.batch.M + token) * a.q_heads + head;
+        // dim 256: the sums of earlier blocks wait in the row's place in memory
+        float *sums = TERMS == 2 && D == 256 ? (alone ? static_cast<float *>(a.out) + token * a.out_stride + (long long)head * D : a.part_o + slot * D) : nullptr;
+        float m = -INFINITY, l = 0.0f, m_sums = -INFINITY;
         bool ok = true;
         for (int blk = first[u], n = 0; blk < last[u]; blk++, n++) {
             const int sb = NQ == 2 ? u : n & 1;
@@ -226,17 +269,28 @@ __global__ void __launch_bounds__(AtShape<D, TERMS>::THREADS, 1) attn_tiles_kern
                 for (int c = 0; c < KEYS; c++)
                     if ((unsigned)(key0 + c - see_lo) >= span) x[c] = -INFINITY;
             }
-            float top = x[0];
+            float tops[8];                                                   // eight chains: one would be 128 dependent steps
 #pragma unroll
-            for (int c = 1; c < KEYS; c++) top = fmaxf(top, x[c]);
-            top *= factor;
+            for (int c = 0; c < 8; c++) tops[c] = fmaxf(x[c], x[c + 8]);
+#pragma unroll
+            for (int c = 16; c < KEYS; c += 16)
+#pragma unroll
+                for (int e = 0; e < 8; e++) tops[e] = fmaxf(fmaxf(tops[e], x[c + e]), x[c + e + 8]);
+            const float top = fmaxf(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])), fmaxf(fmaxf(tops[4], tops[5]), fmaxf(tops[6], tops[7]))) * factor;
+            const bool flush = TERMS == 2 && n > 0 && n % S::FLUSH == 0;
+            if (flush) {
+                if (!mbar_wait_warp(&o_done[0], (uint32_t)(n - 1) & 1u, abort_flag, status, CODE)) { ok = false; break; }
+                tc_fence_after();
+                add_to_sums<D>(lane_base + S::COL_O, lane_base + S::COL_SUM, sums, live, n > S::FLUSH, m_sums == m ? 1.0f : exp2_fast(m_sums - m));
+                m_sums = m;
+            }
             const bool grow = top > m + AT_SLACK;
             if (__any_sync(0xffffffffu, grow)) {
                 const float mn = grow ? top : m;
                 const float f = mn == m ? 1.0f : exp2_fast(m - mn);
                 m = mn;
                 l *= f;
-                if (n > 0) {
+                if (n > 0 && !flush) {
                     // the product of the block before has to be in O: with one score buffer its completion came before these
                     // scores', with two it has a barrier of its own
                     if (NQ == 1) {
@@ -288,10 +342,7 @@ __global__ void __launch_bounds__(AtShape<D, TERMS>::THREADS, 1) attn_tiles_kern
             tc_fence_after();
         }
         if (ok) {
-            const long long token = live ? t.token0 + row / a.group : 0;
-            const int head = kvh * a.group + row % a.group;
-            const long long slot = ((long long)split * a.batch.M + token) * a.q_heads + head;
-            const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+            const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f, sums_by = m_sums == m ? 1.0f : exp2_fast(m_sums - m);
             if (live && !alone) a.part_ml[slot] = make_float2(m, l);
             if (live && alone && a.part_ml) a.part_ml[token * a.q_heads + head] = make_float2(0.0f, -1.0f);
             if (alone || blk1 > blk0) {
@@ -300,6 +351,17 @@ __global__ void __launch_bounds__(AtShape<D, TERMS>::THREADS, 1) attn_tiles_kern
                     float o[32];
                     if (blocks > 0) {
                         at_ld32(o_col + c, o);
+                        if (TERMS == 2 && blocks > S::FLUSH) {
+                            float e[32];
+                            if (D <= 128) at_ld32(lane_base + S::COL_SUM + c, e);
+                            at_wait_ld();
+                            if (D > 128) {
+#pragma unroll
+                                for (int i = 0; i < 32; i++) e[i] = live ? sums[c + i] : 0.0f;
+                            }
+#pragma unroll
+                            for (int i = 0; i < 32; i++) o[i] = fmaf(e[i], sums_by, o[i]);
+                        }
                         at_wait_ld();
                     } else {
 #pragma unroll
@@ -390,7 +452,7 @@ __global__ void __launch_bounds__(AtShape<D, TERMS>::THREADS, 1) attn_tiles_kern
                         wait(&p_full[0], (uint32_t)n & 1u);
                         if (!ok) break;
                         tc_fence_after();
-                        values(0, n & 1, s, n == 0);
+                        values(0, n & 1, s, n % S::FLUSH == 0);
                         umma_commit(&o_done[0]);
                         umma_commit(&kv_empty[s]);
                         next();

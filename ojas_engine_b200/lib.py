@@ -91,7 +91,7 @@ SIGNATURES = {
     "ojas_b200_seqs_check_host": (_i, [_vp, _vp, _vp, _sz, _sz, _sz, _sz, _sz, _sz, _sz, C.c_char_p, _sz]),
     "ojas_b200_kv_append": (_i, [_vp, _vp, _seqs, _vp, _i, _u32, _vp, _sz, _vp, _sz, _vp, _sz, _u32, _vp, _sz, _sz, _vp, _sz]),
     "ojas_b200_kv_append_check": (_i, [_sz, _sz, _sz, _i, _u32, _vp, _sz, _vp, _sz, _vp, _sz, _u32, _vp, _sz, _sz, _vp, _seqs, _sz, C.c_char_p, _sz]),
-    "ojas_b200_attention_workspace_bytes": (_sz, [_vp, _vp, _seqs, _sz, _sz, C.c_longlong]),
+    "ojas_b200_attention_workspace_bytes": (_sz, [_vp, _vp, _seqs, _u32, _sz, _sz, C.c_longlong]),
     "ojas_b200_attention": (_i, [_vp, _vp, _seqs, _u32, _vp, _sz, _sz, _f, _i, C.c_longlong, _vp, _sz, _sz, _vp, _sz]),
     "ojas_b200_attention_check": (_i, [_u32, _sz, _sz, _sz, _u32, _sz, _vp, _sz, _vp, _sz, _f, _i, C.c_longlong, _seqs, _sz, C.c_char_p, _sz]),
     "ojas_b200_gguf_open": (_i, [C.c_char_p, C.POINTER(_vp), C.c_char_p, _sz]),

@@ -294,15 +294,15 @@ class B200Gpu:
                                              k.ptr, x_stride if k_stride is None else k_stride, v.ptr, x_stride if v_stride is None else v_stride,
                                              q_type, q_out.ptr if q_out else None, q_out_stride, q_heads, pos.ptr if pos else None, m))
 
-    def attention_workspace_bytes(self, kv: KvCache, seqs: Seqs, m: int, q_heads: int, window: int = 0) -> int:
-        return int(self._l.ojas_b200_attention_workspace_bytes(self._ctx, kv._h, seqs._ref, m, q_heads, window))
+    def attention_workspace_bytes(self, kv: KvCache, seqs: Seqs, m: int, q_heads: int, act_type: int = F32, window: int = 0) -> int:
+        return int(self._l.ojas_b200_attention_workspace_bytes(self._ctx, kv._h, seqs._ref, act_type, m, q_heads, window))
 
     def attention(self, kv: KvCache, seqs: Seqs, q: Buf, out: Buf, m: int, q_heads: int, act_type: int = F32, scale: float | None = None,
                   causal: bool = True, window: int = 0, q_stride: int = 0, out_stride: int = 0, workspace: Buf | None = None) -> None:
         """Attention of the call's rows over their sequences' keys (scale: 1 / sqrt(dim) unless given).  Without a caller
         workspace a grow-only scratch buffer owned by this object is used; a buffer it outgrew stays allocated, because a
         captured graph may still use it."""
-        need = self._l.ojas_b200_attention_workspace_bytes(self._ctx, kv._h, seqs._ref, m, q_heads, window)
+        need = self._l.ojas_b200_attention_workspace_bytes(self._ctx, kv._h, seqs._ref, act_type, m, q_heads, window)
         if workspace is None and need:
             workspace = self._attn_ws[-1] if self._attn_ws else None
             if workspace is None or workspace.nbytes < need:

@@ -116,7 +116,7 @@ def test_calls_without_a_context_are_refused():
     assert l.ojas_b200_attention(None, None, None, 0, None, 0, 0, 1.0, 1, 0, None, 0, 0, None, 0) == E_ARG
     assert l.ojas_b200_kv_append(None, None, None, None, 0, 0, None, 0, None, 0, None, 0, 0, None, 0, 0, None, 0) == E_ARG
     assert l.ojas_b200_rope_rows(None, None, 0, 0, None, 0, 0, None, 0, None, 0, 0, 0) == E_ARG
-    assert l.ojas_b200_attention_workspace_bytes(None, None, None, 1, 1, 0) == 0
+    assert l.ojas_b200_attention_workspace_bytes(None, None, None, 0, 1, 1, 0) == 0
     l.ojas_b200_kv_destroy(None)
     l.ojas_b200_rope_destroy(None)
 
