@@ -26,6 +26,7 @@ namespace {
 
 constexpr float AT_SHIFT = 8.0f, AT_SLACK = 7.0f;
 constexpr int AT_ROWS = 128;
+constexpr int AT_POLY = 2;                                  // of eight pairs of exponentials, those formed by the polynomial
 
 template <int D, int TERMS>
 struct AtShape {
@@ -36,7 +37,7 @@ struct AtShape {
     static constexpr int STAGES_FIT = (232448 - 1024 - 512 - Q_BYTES) / STAGE;
     static constexpr int STAGES = STAGES_FIT > 6 ? 6 : STAGES_FIT;
     static constexpr int SMEM = Q_BYTES + STAGES * STAGE + 512 + 1024;
-    static constexpr int SOFT_WARPS = 4 * NQ, THREADS = (SOFT_WARPS + 2) * 32;
+    static constexpr int SOFT_WARPS = 4 * NQ, THREADS = (SOFT_WARPS + (NQ == 2 ? 4 : 2)) * 32;   // (NQ 2: whole warpgroups, see the register split)
     static constexpr int COL_S = 0, COL_O = 256, O_STEP = 128;         // TMEM columns: scores, accumulators
     static constexpr int COL_SUM = 384;                                // TERMS 2, dim <= 128: the sums of earlier blocks
     static constexpr int FLUSH = TERMS == 2 ? 512 / KEYS : 1 << 30;    // blocks after which O is added to those sums
@@ -69,24 +70,101 @@ __device__ __forceinline__ void at_st32f(uint32_t taddr, const float *v) {
 }
 __device__ __forceinline__ void at_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// D = A B (accumulate 0) or D += A B; A from shared memory, or from TMEM.
-__device__ __forceinline__ void at_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+// Two f32 operations in one instruction.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+    return v;
 }
-__device__ __forceinline__ void at_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+__device__ __forceinline__ void unpair(uint64_t v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
 }
-// kind::f16: f32 accumulator, M = 128, N = n; `mn`: B is stored with N contiguous (the rows of V).
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {       // NaN if any is
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// 2^y of two values on the multiply-add units: y = j + f, |f| <= 1/2, 2^f by a polynomial of degree 4 (least largest relative error
+// on that interval, 2.7e-6; P is rounded to 2^-12 or more), j added to the exponent.  The special-function unit gives 16 exponentials
+// a cycle per SM, as long for a tile's scores as the tensor cores need for both its products: a part is formed here instead.
+// Below 2^-126 the result is about 2^-126.
+__device__ __forceinline__ void exp2_poly(uint64_t y, float &p0, float &p1) {
+    float a, b;
+    unpair(y, a, b);
+    y = pair(fmaxf(a, -126.0f), fmaxf(b, -126.0f));
+    const uint64_t magic = pair(12582912.0f, 12582912.0f), unmagic = pair(-12582912.0f, -12582912.0f);   // 1.5 * 2^23: rounds to whole numbers
+    const uint64_t r = add2(y, magic), f = fma2(add2(r, unmagic), pair(-1.0f, -1.0f), y);
+    uint64_t p = fma2(pair(0.009570101276040077f, 0.009570101276040077f), f, pair(0.05591785907745361f, 0.05591785907745361f));
+    p = fma2(p, f, pair(0.240247443318367f, 0.240247443318367f));
+    p = fma2(p, f, pair(0.6931217908859253f, 0.6931217908859253f));
+    p = fma2(p, f, pair(0.9999992847442627f, 0.9999992847442627f));
+    float r0, r1;
+    unpair(p, p0, p1);
+    unpair(r, r0, r1);
+    p0 = __int_as_float(__float_as_int(p0) + (__float_as_int(r0) << 23));
+    p1 = __int_as_float(__float_as_int(p1) + (__float_as_int(r1) << 23));
+}
+
+// Bounded wait without a call (ptxas splits registers between the roles only in code without calls).  Whole warps or one thread.
+__device__ __forceinline__ bool at_wait(uint64_t *bar, uint32_t parity, volatile int *abort_flag, unsigned *status) {
+    if (mbar_test(bar, parity)) return true;
+    const long long t0 = clock64();
+    while (!mbar_try(bar, parity)) {
+        if (*abort_flag) return false;
+        if (clock64() - t0 > WAIT_CYCLES) {
+            *abort_flag = 1;
+            atomicOr(status, OJAS_ST_ATTN_WAIT);
+            __threadfence_system();
+            return false;
+        }
+    }
+    return true;
+}
+__device__ __forceinline__ bool at_wait_warp(uint64_t *bar, uint32_t parity, volatile int *abort_flag, unsigned *status) {
+    return __all_sync(0xffffffffu, at_wait(bar, parity, abort_flag, status));
+}
+
+// One lane of a converged warp, chosen by the hardware: the compiler then knows that one thread issues what follows.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(ok));
+    return ok != 0;
+}
+
+// Shared-memory operands: the upper word of the descriptor is the same for all of them (groups of eight rows 1024 bytes apart,
+// version 1, 128-byte swizzle), the lower one holds the address and, for V, the distance of its 64-column slabs.
+constexpr uint32_t AT_DESC_HI = (1024u >> 4) | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint32_t at_desc(uint32_t smem_addr, uint32_t slab) { return ((smem_addr & 0x3FFFFu) >> 4) | (slab >> 4) << 16; }
+// D = A B (accumulate 0) or D += A B; A from shared memory, or from TMEM.  The issuing warp shares its scheduler with two softmax
+// warps: what it does per instruction has to stay below the 64 cycles an instruction takes, so the operands are kept where the
+// compiler sees that they are the same in all lanes.
+__device__ __forceinline__ void at_mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tmov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(AT_DESC_HI) : "memory");
+}
+__device__ __forceinline__ void at_mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 db;\n\tmov.b64 db, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(AT_DESC_HI) : "memory");
+}
+// kind::f16: f32 accumulator, M = 128, N = n; `mn`: B is stored with N contiguous (the rows of V: dim).
 __host__ __device__ constexpr uint32_t at_idesc(int n, bool bf, bool mn) {
     return (1u << 4) | (bf ? (1u << 7) | (1u << 10) : 0u) | (mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(AT_ROWS >> 4) << 24);
 }
-// V as B operand: N (dim) contiguous, 128-byte swizzle; slabs of 64 columns `slab` bytes apart, groups of eight keys 1024 bytes.
-__device__ __forceinline__ uint64_t at_desc_mn(uint32_t smem_addr, uint32_t slab) {
-    return (uint64_t)((smem_addr & 0x3FFFFu) >> 4) | (uint64_t)(slab >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
-}
-
 // sums = sums * by + O (first time: sums = O) for this thread's row, and O may be overwritten.
 template <int D>
 __device__ __forceinline__ void add_to_sums(uint32_t o_col, uint32_t sum_col, float *sums, bool live, bool more, float by) {
@@ -184,15 +262,15 @@ __global__ void __launch_bounds__(AtShape<D, TERMS>::THREADS, 1) attn_tiles_kern
     uint64_t *kv_full = bars, *kv_empty = bars + 8, *s_full = bars + 16, *p_full = bars + 18, *o_done = bars + 20, *q_full = bars + 22, *raw = bars + 24;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 26);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kvh = blockIdx.y, split = blockIdx.z;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, split = blockIdx.z;
+    const int kv_heads = a.q_heads / a.group, kvh = blockIdx.x % kv_heads;
     unsigned *status = a.batch.status;
-    constexpr unsigned CODE = OJAS_ST_ATTN_WAIT;
 
     grid_launch_dependents();
     grid_dependency_wait();
-    // long tiles first: the last rows of a sequence see the most keys
+    // long tiles first, of all heads: the last rows of a sequence see the most keys
     RowTile t;
-    if (!find_tile(a, gridDim.x - 1 - blockIdx.x, NQ * AT_ROWS, lane, t)) return;
+    if (!find_tile(a, (gridDim.x - 1 - blockIdx.x) / kv_heads, NQ * AT_ROWS, lane, t)) return;
     const int rows = min(NQ * AT_ROWS, t.n_rows - t.row0);
     int lo, hi;
     key_range(a, t, t.row0, t.row0 + rows, lo, hi);
@@ -231,7 +309,9 @@ __global__ void __launch_bounds__(AtShape<D, TERMS>::THREADS, 1) attn_tiles_kern
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
+    // Register split (NQ 2): 384 threads are launched with 168 registers each; 2 * 224 + 56 = 3 * 168.
     if (warp < S::SOFT_WARPS) {
+        if (NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         // ---------------- softmax of tile u: thread = row
         const int u = warp >> 2, quarter = warp & 3;
         const int r0 = t.row0 + u * AT_ROWS, row = r0 + quarter * 32 + lane;
@@ -251,19 +331,58 @@ __global__ void __launch_bounds__(AtShape<D, TERMS>::THREADS, 1) attn_tiles_kern
         const long long slot = ((long long)split * a.batch.M + token) * a.q_heads + head;
         // dim 256: the sums of earlier blocks wait in the row's place in memory
         float *sums = TERMS == 2 && D == 256 ? (alone ? static_cast<float *>(a.out) + token * a.out_stride + (long long)head * D : a.part_o + slot * D) : nullptr;
-        float m = -INFINITY, l = 0.0f, m_sums = -INFINITY;
+        float m = live ? -INFINITY : 0.0f, l = 0.0f, m_sums = -INFINITY;   // (rows past the tile's last only keep out of the way)
         bool ok = true;
         for (int blk = first[u], n = 0; blk < last[u]; blk++, n++) {
             const int sb = NQ == 2 ? u : n & 1;
             const uint32_t s_col = lane_base + S::COL_S + sb * 128;
-            if (!mbar_wait_warp(&s_full[sb], NQ == 2 ? (uint32_t)n & 1u : (uint32_t)(n >> 1) & 1u, abort_flag, status, CODE)) { ok = false; break; }
+            if (!at_wait_warp(&s_full[sb], NQ == 2 ? (uint32_t)n & 1u : (uint32_t)(n >> 1) & 1u, abort_flag, status)) { ok = false; break; }
             tc_fence_after();
             float x[KEYS];
 #pragma unroll
             for (int c = 0; c < KEYS; c += 32) at_ld32(s_col + c, x + c);
             at_wait_ld();
             const int key0 = blk * KEYS;
-            if (__any_sync(0xffffffffu, key0 < see_lo || key0 + KEYS > see_hi)) {
+            // Most blocks raise no row's maximum by more than the slack: their probabilities are formed against the maximum so far
+            // while the block's own is still being looked for, and only kept if it is within the slack (NaN is not).
+            const bool flush = TERMS == 2 && n > 0 && n % S::FLUSH == 0;
+            const bool edge = __any_sync(0xffffffffu, live && (key0 < see_lo || key0 + KEYS > see_hi));
+            bool done = false;
+            if (TERMS == 1 && !__any_sync(0xffffffffu, edge || (live && m == -INFINITY))) {
+                const uint64_t by = pair(factor, factor), less = pair(AT_SHIFT - m, AT_SHIFT - m);
+                uint64_t sum[2] = {0ull, 0ull};
+                float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int c = 0; c < KEYS; c += 32) {
+                    uint32_t p16[16];
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const float x0 = x[c + 2 * i], x1 = x[c + 2 * i + 1];
+                        const uint64_t y = fma2(pair(x0, x1), by, less);
+                        float p0, p1;
+                        if (i % 8 < AT_POLY) {
+                            exp2_poly(y, p0, p1);
+                        } else {
+                            unpair(y, p0, p1);
+                            p0 = exp2_fast(p0);
+                            p1 = exp2_fast(p1);
+                        }
+                        tops[i & 3] = max3_nan(tops[i & 3], x0, x1);
+                        sum[i & 1] = add2(sum[i & 1], pair(p0, p1));
+                        p16[i] = pack_half(p0, p1, BF);
+                    }
+                    at_st16(s_col + c / 2, p16);
+                }
+                const float top = max3_nan(max3_nan(tops[0], tops[1], tops[2]), tops[3], tops[3]) * factor;
+                done = __all_sync(0xffffffffu, top <= m + AT_SLACK || !live);
+                if (done) {
+                    float s0, s1;
+                    unpair(add2(sum[0], sum[1]), s0, s1);
+                    l += s0 + s1;
+                }
+            }
+            if (!done) {
+            if (edge) {
                 const unsigned span = (unsigned)max(0, see_hi - see_lo);
 #pragma unroll
                 for (int c = 0; c < KEYS; c++)
@@ -275,11 +394,10 @@ __global__ void __launch_bounds__(AtShape<D, TERMS>::THREADS, 1) attn_tiles_kern
 #pragma unroll
             for (int c = 16; c < KEYS; c += 16)
 #pragma unroll
-                for (int e = 0; e < 8; e++) tops[e] = fmaxf(fmaxf(tops[e], x[c + e]), x[c + e + 8]);
-            const float top = fmaxf(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])), fmaxf(fmaxf(tops[4], tops[5]), fmaxf(tops[6], tops[7]))) * factor;
-            const bool flush = TERMS == 2 && n > 0 && n % S::FLUSH == 0;
+                for (int e = 0; e < 8; e++) tops[e] = max3(tops[e], x[c + e], x[c + e + 8]);
+            const float top = max3(max3(tops[0], tops[1], tops[2]), max3(tops[3], tops[4], tops[5]), fmaxf(tops[6], tops[7])) * factor;
             if (flush) {
-                if (!mbar_wait_warp(&o_done[0], (uint32_t)(n - 1) & 1u, abort_flag, status, CODE)) { ok = false; break; }
+                if (!at_wait_warp(&o_done[0], (uint32_t)(n - 1) & 1u, abort_flag, status)) { ok = false; break; }
                 tc_fence_after();
                 add_to_sums<D>(lane_base + S::COL_O, lane_base + S::COL_SUM, sums, live, n > S::FLUSH, m_sums == m ? 1.0f : exp2_fast(m_sums - m));
                 m_sums = m;
@@ -294,7 +412,7 @@ __global__ void __launch_bounds__(AtShape<D, TERMS>::THREADS, 1) attn_tiles_kern
                     // the product of the block before has to be in O: with one score buffer its completion came before these
                     // scores', with two it has a barrier of its own
                     if (NQ == 1) {
-                        if (!mbar_wait_warp(&o_done[0], (uint32_t)(n - 1) & 1u, abort_flag, status, CODE)) { ok = false; break; }
+                        if (!at_wait_warp(&o_done[0], (uint32_t)(n - 1) & 1u, abort_flag, status)) { ok = false; break; }
                         tc_fence_after();
                     }
 #pragma unroll 1
@@ -327,10 +445,11 @@ __global__ void __launch_bounds__(AtShape<D, TERMS>::THREADS, 1) attn_tiles_kern
                 if (TERMS == 2) at_st16(s_col + KEYS / 2 + c / 2, lo16);
             }
             l += (part[0] + part[1]) + (part[2] + part[3]);
+            }
             at_wait_st();
             // With two score buffers the scores run a block ahead: passing these probabilities on only when the product before has
             // ended keeps every waiter within one phase of its barrier (a parity cannot tell a phase from the one two before).
-            if (NQ == 1 && n > 0 && !mbar_wait_warp(&o_done[0], (uint32_t)(n - 1) & 1u, abort_flag, status, CODE)) { ok = false; break; }
+            if (NQ == 1 && n > 0 && !at_wait_warp(&o_done[0], (uint32_t)(n - 1) & 1u, abort_flag, status)) { ok = false; break; }
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&p_full[u]);
@@ -338,7 +457,7 @@ __global__ void __launch_bounds__(AtShape<D, TERMS>::THREADS, 1) attn_tiles_kern
         // ---------------- the tile's rows: O / l to out, or O and (m, l) to the split's place
         const int blocks = last[u] - first[u];
         if (ok && blocks > 0) {
-            ok = mbar_wait_warp(&o_done[u], NQ == 2 ? 0u : (uint32_t)(blocks - 1) & 1u, abort_flag, status, CODE);
+            ok = at_wait_warp(&o_done[u], NQ == 2 ? 0u : (uint32_t)(blocks - 1) & 1u, abort_flag, status);
             tc_fence_after();
         }
         if (ok) {
@@ -379,108 +498,132 @@ __global__ void __launch_bounds__(AtShape<D, TERMS>::THREADS, 1) attn_tiles_kern
                 }
             }
         }
-    } else if (warp == S::SOFT_WARPS) {
-        // ---------------- MMA issue (one thread); ring order: see the loader
-        if (lane == 0) {
-            constexpr uint32_t ID_S = at_idesc(KEYS, BF, false), ID_O = at_idesc(D, BF, true);
-            bool ok = true;
-            int s = 0;
-            uint32_t phase = 0;
-            auto next = [&]() { if (++s == STAGES) { s = 0; phase ^= 1u; } };
-            auto wait = [&](uint64_t *bar, uint32_t parity) { ok = ok && mbar_wait_spin(bar, parity, abort_flag, status, CODE); };
-            auto scores = [&](int u, int buf, int stage) {
-                const uint64_t kd = umma_desc(smem_u32(ring + stage * STAGE));
+    } else {
+    if (NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == S::SOFT_WARPS) {
+        // ---------------- MMA issue: the warp waits together, one elected lane issues.  Ring order: see the loader
+        constexpr uint32_t ID_S = at_idesc(KEYS, BF, false), ID_O = at_idesc(D, BF, true);
+        bool ok = true;
+        const int b0 = __shfl_sync(0xffffffffu, blk0, 0), b1 = __shfl_sync(0xffffffffu, blk1, 0);
+        int from[NQ], to[NQ];
 #pragma unroll
-                for (int term = 0; term < TERMS; term++) {
-                    const uint64_t qd = umma_desc(smem_u32(smem + (u * TERMS + term) * S::Q_TERM));
+        for (int u = 0; u < NQ; u++) { from[u] = __shfl_sync(0xffffffffu, first[u], 0); to[u] = __shfl_sync(0xffffffffu, last[u], 0); }
+        int s = 0;
+        uint32_t phase = 0;
+        const uint32_t ring_at = __shfl_sync(0xffffffffu, smem_u32(ring), 0), q_at = __shfl_sync(0xffffffffu, smem_u32(smem), 0);
+        const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+        auto next = [&]() { if (++s == STAGES) { s = 0; phase ^= 1u; } };
+        auto wait = [&](uint64_t *bar, uint32_t parity) { ok = ok && at_wait_warp(bar, parity, abort_flag, status); };
+        auto scores = [&](int u, int buf, int stage) {
+            const uint32_t kd = at_desc(ring_at + stage * STAGE, 16);
 #pragma unroll
-                    for (int k = 0; k < D / 16; k++)     // 16 of dim: 32 bytes of a row, four per slab
-                        at_mma_ss(tmem + S::COL_S + buf * 128, qd + (k >> 2) * (AT_ROWS * 128 / 16) + (k & 3) * 2, kd + (k >> 2) * (KEYS * 128 / 16) + (k & 3) * 2, ID_S,
-                                  term + k > 0);
-                }
-                umma_commit(&s_full[buf]);
-            };
-            auto values = [&](int u, int buf, int stage, bool begin) {
-                const uint64_t vd = at_desc_mn(smem_u32(ring + stage * STAGE), KEYS * 128);
+            for (int term = 0; term < TERMS; term++) {     // the low term first, while the sums are small
+                const uint32_t qd = at_desc(q_at + (u * TERMS + TERMS - 1 - term) * S::Q_TERM, 16);
 #pragma unroll
-                for (int term = 0; term < TERMS; term++)
+                for (int k = 0; k < D / 16; k++)           // 16 of dim: 32 bytes of a row, four per slab
+                    at_mma_ss(tm + S::COL_S + buf * 128, qd + (k >> 2) * (AT_ROWS * 128 / 16) + (k & 3) * 2, kd + (k >> 2) * (KEYS * 128 / 16) + (k & 3) * 2, ID_S,
+                              term + k > 0);
+            }
+            umma_commit(&s_full[buf]);
+        };
+        auto values = [&](int u, int buf, int stage, bool begin) {
+            const uint32_t vd = at_desc(ring_at + stage * STAGE, KEYS * 128);
 #pragma unroll
-                    for (int k = 0; k < KEYS / 16; k++)  // 16 keys: 8 columns of packed P, 2048 bytes of V
-                        at_mma_ts(tmem + S::COL_O + u * S::O_STEP, tmem + S::COL_S + buf * 128 + term * (KEYS / 2) + k * 8, vd + k * (2048 / 16), ID_O, !begin || term + k > 0);
-            };
-            for (int u = 0; u < NQ; u++)
-                if (last[u] > first[u]) wait(&q_full[u], 0);
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            if (NQ == 2) {
-                int v_stage = 0, n[2] = {0, 0};
-                for (int i = blk0; ok && i <= blk1; i++) {
-                    // block i's K is at the ring's head, block i - 1's V one behind it: (K0) (V0 K1) (V1 K2) ... (Vlast)
-                    if (i > blk0) { wait(&kv_full[s], phase); v_stage = s; next(); }
-                    const int k_stage = s;
-                    if (i < blk1) { wait(&kv_full[s], phase); next(); }
+            for (int term = 0; term < TERMS; term++)
+#pragma unroll
+                for (int k = 0; k < KEYS / 16; k++)        // 16 keys: 8 columns of packed P, 2048 bytes of V
+                    at_mma_ts(tm + S::COL_O + u * S::O_STEP, tm + S::COL_S + buf * 128 + term * (KEYS / 2) + k * 8, vd + k * (2048 / 16), ID_O, !begin || term + k > 0);
+        };
+        for (int u = 0; u < NQ; u++)
+            if (to[u] > from[u]) wait(&q_full[u], 0);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        if (NQ == 2) {
+            int v_stage = 0, n[2] = {0, 0};
+            for (int i = b0; ok && i <= b1; i++) {
+                // block i's K is at the ring's head, block i - 1's V one behind it: (K0) (V0 K1) (V1 K2) ... (Vlast)
+                if (i > b0) { wait(&kv_full[s], phase); v_stage = s; next(); }
+                const int k_stage = s;
+                const uint32_t k_phase = phase;
+                if (i < b1) next();
+#pragma unroll
+                for (int u = 0; u < NQ; u++) {
+                    const bool has_v = i - 1 >= from[u] && i - 1 < to[u], has_k = i >= from[u] && i < to[u];
+                    if (has_v) {
+                        wait(&p_full[u], (uint32_t)n[u] & 1u);
+                        if (!ok) break;
+                        tc_fence_after();
+                    }
+                    if (elect_one()) {
+                        if (has_v) {
+                            values(u, u, v_stage, n[u] == 0);
+                            if (i == to[u]) umma_commit(&o_done[u]);
+                        }
+                        if (u == NQ - 1 && i > b0) umma_commit(&kv_empty[v_stage]);
+                    }
+                    __syncwarp();
+                    if (u == 0 && i < b1) wait(&kv_full[k_stage], k_phase);
                     if (!ok) break;
                     tc_fence_after();
-#pragma unroll
-                    for (int u = 0; u < NQ; u++) {
-                        if (i - 1 >= first[u] && i - 1 < last[u]) {
-                            wait(&p_full[u], (uint32_t)n[u] & 1u);
-                            if (!ok) break;
-                            tc_fence_after();
-                            values(u, u, v_stage, n[u] == 0);
-                            n[u]++;
-                            if (i == last[u]) umma_commit(&o_done[u]);
-                        }
-                        if (u == NQ - 1 && i > blk0) umma_commit(&kv_empty[v_stage]);
-                        if (i >= first[u] && i < last[u]) scores(u, u, k_stage);
-                        if (u == NQ - 1 && i < blk1) umma_commit(&kv_empty[k_stage]);
+                    if (elect_one()) {
+                        if (has_k) scores(u, u, k_stage);
+                        if (u == NQ - 1 && i < b1) umma_commit(&kv_empty[k_stage]);
                     }
+                    __syncwarp();
+                    n[u] += has_v;
                 }
-            } else {
-                for (int i = blk0; ok && i <= blk1; i++) {
-                    // (K0) (K1 V0) (K2 V1) ... (Vlast)
-                    if (i < blk1) {
-                        wait(&kv_full[s], phase);
-                        if (!ok) break;
-                        tc_fence_after();
-                        scores(0, (i - blk0) & 1, s);
+            }
+        } else {
+            for (int i = b0; ok && i <= b1; i++) {
+                // (K0) (K1 V0) (K2 V1) ... (Vlast)
+                if (i < b1) {
+                    wait(&kv_full[s], phase);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (elect_one()) {
+                        scores(0, (i - b0) & 1, s);
                         umma_commit(&kv_empty[s]);
-                        next();
                     }
-                    if (i > blk0) {
-                        const int n = i - 1 - blk0;
-                        wait(&kv_full[s], phase);
-                        wait(&p_full[0], (uint32_t)n & 1u);
-                        if (!ok) break;
-                        tc_fence_after();
+                    __syncwarp();
+                    next();
+                }
+                if (i > b0) {
+                    const int n = i - 1 - b0;
+                    wait(&kv_full[s], phase);
+                    wait(&p_full[0], (uint32_t)n & 1u);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (elect_one()) {
                         values(0, n & 1, s, n % S::FLUSH == 0);
                         umma_commit(&o_done[0]);
                         umma_commit(&kv_empty[s]);
-                        next();
                     }
+                    __syncwarp();
+                    next();
                 }
             }
         }
-    } else {
+    } else if (warp == S::SOFT_WARPS + 1) {
         // ---------------- loader: lane = one box (64 values x box_rows tokens).  NQ 2: K0 V0 K1 V1 ...; NQ 1: K0 K1 V0 K2 V1 ...
-        const int per_slab = KEYS / box_rows, boxes = per_slab * (D / 64);
+        const int per_slab = KEYS / box_rows, part = lane % per_slab, slab = lane / per_slab;
+        const bool has_box = slab < D / 64;
+        const int *table = a.batch.table + (long long)t.seq * a.batch.table_stride;
+        const int page_size = a.batch.page_size, step_entry = KEYS / page_size, step_slot = KEYS - step_entry * page_size;
         int s = 0;
         uint32_t phase = 1, raw_phase = 0;
-        const int n = blk1 - blk0;
         bool ok = true;
-        for (int i = 0; ok && i < 2 * n; i++) {
-            // the i-th block of the ring: which block, K or V
-            const bool is_v = NQ == 2 ? (i & 1) : i == 2 * n - 1 || (i >= 2 && (i & 1) == 0);
-            const int b = NQ == 2 ? i >> 1 : is_v ? (i == 2 * n - 1 ? n - 1 : i / 2 - 1) : (i + 1) / 2;
-            const int blk = blk0 + b;
-            if (!mbar_wait_warp(&kv_empty[s], phase, abort_flag, status, CODE)) break;
+        // this lane's box of block blk: the page (looked up a block ahead of its use, -1: not needed) and the token in it
+        int key = blk0 * KEYS + part * box_rows, entry = key / page_size, slot = key - entry * page_size;
+        auto look_up = [&]() { return has_box && key < hi && key + box_rows > lo ? __ldg(table + entry) : -1; };
+        auto advance = [&]() {
+            key += KEYS;
+            entry += step_entry;
+            slot += step_slot;
+            if (slot >= page_size) { slot -= page_size; entry++; }
+        };
+        auto copy = [&](const CUtensorMap *map, bool is_v, int blk, bool want, int page, int at) {
+            ok = ok && at_wait_warp(&kv_empty[s], phase, abort_flag, status);
+            if (!ok) return;
             unsigned char *to = ring + s * STAGE;
-            const int part = lane % per_slab, slab = lane / per_slab, key = blk * KEYS + part * box_rows;
-            const bool want = lane < boxes && key < hi && key + box_rows > lo;
-            int page = 0;
-            if (want) {
-                page = __ldg(a.batch.table + (long long)t.seq * a.batch.table_stride + key / a.batch.page_size);
-                if (page < 0 || page >= a.batch.pages) { atomicOr(status, OJAS_ST_BATCH); page = a.batch.pages; }      // reads as zeros
-            }
             const int copies = __popc(__ballot_sync(0xffffffffu, want));
             // the values of keys that are not read must be zeros (0 * NaN is NaN): such a block lands on a barrier of the loader's own
             // and is passed on after they are
@@ -488,10 +631,9 @@ __global__ void __launch_bounds__(AtShape<D, TERMS>::THREADS, 1) attn_tiles_kern
             uint64_t *bar = edge ? raw : &kv_full[s];
             if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(copies * box_rows * 128));
             __syncwarp();
-            if (want)
-                tma_load_4d(to + slab * (KEYS * 128) + part * box_rows * 128, is_v ? &map_v : &map_k, slab * 64, key % a.batch.page_size, kvh, page, bar);
+            if (want) tma_load_4d(to + slab * (KEYS * 128) + part * box_rows * 128, map, slab * 64, at, kvh, page, bar);
             if (edge) {
-                ok = mbar_wait_warp(raw, raw_phase, abort_flag, status, CODE);
+                ok = at_wait_warp(raw, raw_phase, abort_flag, status);
                 raw_phase ^= 1u;
                 for (int e = lane; e < KEYS * (D / 8); e += 32) {          // 16-byte pieces; a row's pieces may be zeroed in any order
                     const int r = e / (D / 8), c = e % (D / 8);
@@ -502,7 +644,23 @@ __global__ void __launch_bounds__(AtShape<D, TERMS>::THREADS, 1) attn_tiles_kern
                 if (lane == 0) mbar_arrive(&kv_full[s]);
             }
             if (++s == STAGES) { s = 0; phase ^= 1u; }
+        };
+        int next_page = blk0 < blk1 ? look_up() : -1, v_page = 0, v_slot = 0;
+        bool v_want = false;
+        for (int blk = blk0; blk < blk1 && ok; blk++) {
+            const bool want = has_box && key < hi && key + box_rows > lo;
+            int page = next_page;
+            const int at = slot;
+            if (want && (page < 0 || page >= a.batch.pages)) { atomicOr(status, OJAS_ST_BATCH); page = a.batch.pages; }   // reads as zeros
+            advance();
+            if (blk + 1 < blk1) next_page = look_up();
+            copy(&map_k, false, blk, want, page, at);
+            if (NQ == 2) copy(&map_v, true, blk, want, page, at);
+            else if (blk > blk0) copy(&map_v, true, blk - 1, v_want, v_page, v_slot);
+            v_want = want; v_page = page; v_slot = at;
         }
+        if (NQ == 1 && blk1 > blk0) copy(&map_v, true, blk1 - 1, v_want, v_page, v_slot);
+    }
     }
 
     // ---------------- teardown: every role arrives here, also after an abort (copies and MMAs in flight then get a bounded time)
@@ -524,7 +682,7 @@ cudaError_t launch_tiles(const ojas_b200_ctx *ctx, const ojas_b200_kv *kv, const
     cudaError_t e = cudaFuncSetAttribute(attn_tiles_kernel<D, BF, TERMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)p.tiles, (unsigned)kv->heads, (unsigned)p.splits);
+    cfg.gridDim = dim3((unsigned)(p.tiles * (long long)kv->heads), 1, (unsigned)p.splits);
     cfg.blockDim = dim3(S::THREADS);
     cfg.dynamicSmemBytes = S::SMEM;
     cfg.stream = ctx->stream;
