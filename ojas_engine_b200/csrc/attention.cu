@@ -360,6 +360,7 @@ static int attn_shape_check(uint32_t cache_type, size_t page_size, size_t kv_hea
     return 0;
 }
 
+constexpr double PLAN_FIXED = 3.0, PLAN_JOIN = 3.0;          // in key blocks
 // Which kernel, and how far the keys are split so that few rows still use every SM.
 static AttnPlan attn_plan(int sm_count, size_t n_seqs, size_t M, size_t max_rows, size_t max_len, size_t q_heads, size_t kv_heads, size_t dim, size_t window, bool f32) {
     AttnPlan p{};
@@ -372,15 +373,19 @@ static AttnPlan attn_plan(int sm_count, size_t n_seqs, size_t M, size_t max_rows
     p.tiles = (long long)(by_seq < by_row ? by_seq : by_row);
     size_t span = max_len;                                   // keys a tile can see at most
     if (window && window + p.rows < span) span = window + p.rows;
-    const size_t blocks = span / p.block + 2;
-    const long long slots = (long long)sm_count * (dim == 256 || p.tensor ? 1 : 2), ctas = p.tiles * (long long)kv_heads;
-    long long want = p.tensor ? slots / ctas : ctas >= 4 * slots ? 1 : (2 * slots + ctas - 1) / ctas;
-    const long long most = (long long)((blocks + 3) / 4);    // a split of fewer than 4 blocks costs more to start and join than it saves
-    if (want > most) want = most;
-    if (want > 1024) want = 1024;
-    if (want < 1) want = 1;
-    p.split_blocks = (int)((blocks + want - 1) / want);
-    p.splits = (int)((blocks + p.split_blocks - 1) / p.split_blocks);
+    const double blocks = (double)(span / p.block + 2), ctas = (double)p.tiles * (double)kv_heads;
+    // A CTA costs its start and end (about as long as `fixed` key blocks) and its blocks; CTAs are handed to `slots` places as
+    // they come free, so that the last of them ends about half a CTA after the work would on average; joining costs a launch.
+    const double slots = (double)sm_count * (dim == 256 || p.mt == 2 || p.tensor ? 1 : 2), fixed = PLAN_FIXED;
+    double best = 0.0;
+    int splits = 1;
+    for (int n = 1; n <= 64 && n * 2 <= (int)blocks; n = n < 8 ? n + 1 : n + n / 4) {
+        const double each = fixed + blocks / n, all = ctas * n;
+        const double cost = (all <= slots ? each : all * each / slots + 0.5 * each) + (n > 1 ? PLAN_JOIN : 0.0);
+        if (n == 1 || cost < best) { best = cost; splits = n; }
+    }
+    p.split_blocks = (int)((blocks + splits - 1) / splits);
+    p.splits = (int)(((long long)blocks + p.split_blocks - 1) / p.split_blocks);
     const size_t rows = M * q_heads;
     p.workspace = p.splits > 1 ? align256((size_t)p.splits * rows * sizeof(float2)) + (size_t)p.splits * rows * dim * sizeof(float) : 0;
     return p;

@@ -3,14 +3,17 @@
 //
 // A CTA takes NQ tiles of 128 rows (rows = token * group + head in group, so a short chunk still fills tiles) of one key head and a
 // range of key blocks.  One warp copies K and V blocks from the pages into a ring (tensor copies, 128-byte swizzle), one thread
-// issues the MMAs, and four warps per tile do the softmax: thread = row = TMEM lane, its scores come out of TMEM into
-// registers, the running maximum and sum stay in registers, and the probabilities go back into TMEM over the scores they came
-// from, where the second product reads them as its A operand.  Q stays in shared memory, O in TMEM.
-//   NQ = 2 (dim 64 and 128, 16-bit activations): while one tile's softmax runs the tensor cores work for the other tile.
-//   NQ = 1 (dim 256, whose O takes half of TMEM, and f32 activations): two score buffers; the next block's scores are formed
-//          while the softmax runs.
-// The accumulator is rescaled only when a row's maximum has grown by more than 2^AT_SLACK since it was last fixed (rare after
-// the first blocks): probabilities are kept scaled by 2^AT_SHIFT and stay below f16's limit and above its smallest values.
+// issues the MMAs, and four warps per tile (NQ 1: eight) do the softmax: thread = row = TMEM lane (NQ 1: two threads to a row), its scores come out of TMEM into
+// registers, the running maximum and sum stay in registers, and the probabilities go back into TMEM, where the second product
+// reads them as its A operand.  Q stays in shared memory, O in TMEM.
+//   NQ = 2 (dim 64 and 128, 16-bit activations): while one tile's softmax runs the tensor cores work for the other tile.  (Blocks of
+//          64 keys would leave TMEM for probabilities beside the scores and let the scores run ahead, but every group of MMAs with a
+//          completion signal takes 300 cycles at least and N = 64 is bound by shared memory: 828 against 565 us for an 8192-token prompt.)
+//   NQ = 1 (dim 256, whose O takes half of TMEM, and f32 activations): two score buffers, whose columns the probabilities reuse;
+//          the next block's scores are formed while the softmax runs.
+// The accumulator is rescaled only when a row's maximum has grown by more than AT_SLACK (in log2) since it was last fixed, or a
+// block's probabilities would leave f16's range (rare after the first blocks): they are kept scaled by 2^AT_SHIFT, below
+// f16's limit and above its smallest values.
 //
 // f32 activations enter as two 16-bit terms (TERMS = 2): Q = Qhi + Qlo against the same K, P = Phi + Plo against the same V, twice the
 // MMAs; rows of q are scaled by a power of two so that both terms are in f16's range.  16-bit activations are exact as they
@@ -25,22 +28,32 @@
 namespace {
 
 constexpr float AT_SHIFT = 8.0f, AT_SLACK = 7.0f;
+constexpr float AT_SUM_MOST = 49152.0f;                    // (a block of 128 scores at the maximum gives 128 * 2^AT_SHIFT = 32768)
 constexpr int AT_ROWS = 128;
+constexpr int AT_MAX_STAGES = 10;
 constexpr int AT_POLY = 2;                                  // of eight pairs of exponentials, those formed by the polynomial
 
 template <int D, int TERMS>
 struct AtShape {
     static constexpr int NQ = D == 256 || TERMS == 2 ? 1 : 2;          // row tiles of a CTA
     static constexpr int KEYS = D == 256 ? 64 : 128;                   // keys of a block
+    static constexpr bool AHEAD = NQ == 1;                             // a block's scores are formed before the products of the one before
     static constexpr int STAGE = KEYS * D * 2;                         // one block of K or V
     static constexpr int Q_TERM = AT_ROWS * D * 2, Q_BYTES = NQ * TERMS * Q_TERM;
-    static constexpr int STAGES_FIT = (232448 - 1024 - 512 - Q_BYTES) / STAGE;
-    static constexpr int STAGES = STAGES_FIT > 6 ? 6 : STAGES_FIT;
-    static constexpr int SMEM = Q_BYTES + STAGES * STAGE + 512 + 1024;
-    static constexpr int SOFT_WARPS = 4 * NQ, THREADS = (SOFT_WARPS + (NQ == 2 ? 4 : 2)) * 32;   // (NQ 2: whole warpgroups, see the register split)
-    static constexpr int COL_S = 0, COL_O = 256, O_STEP = 128;         // TMEM columns: scores, accumulators
-    static constexpr int COL_SUM = 384;                                // TERMS 2, dim <= 128: the sums of earlier blocks
-    static constexpr int FLUSH = TERMS == 2 ? 512 / KEYS : 1 << 30;    // blocks after which O is added to those sums
+    static constexpr int SHARE = NQ == 1 ? 2 : 1;                      // threads that share a row: one tile alone needs eight warps to hide latencies
+    static constexpr int SMALL = 512 + (SHARE == 2 ? 2 * AT_ROWS * 4 : 0);           // barriers, and what the two threads of a row tell each other
+    static constexpr int STAGES_FIT = (232448 - 1024 - SMALL - Q_BYTES) / STAGE;
+    static constexpr int STAGES = STAGES_FIT > AT_MAX_STAGES ? AT_MAX_STAGES : STAGES_FIT;
+    static constexpr int SMEM = Q_BYTES + STAGES * STAGE + SMALL + 1024;
+    static constexpr int COLS = KEYS / SHARE, OUT = D / SHARE;         // scores, and columns of O, of a softmax thread
+    static constexpr int SOFT_WARPS = 4 * NQ * SHARE, THREADS = (SOFT_WARPS + (NQ == 2 ? 4 : 2)) * 32;   // (NQ 2: whole warpgroups, see the register split)
+    // TMEM columns: scores (NQ 1: two buffers), whose columns the probabilities reuse; O; (TERMS 2, dim <= 128) the sums of earlier blocks.
+    static constexpr int FLUSH = TERMS == 2 ? 512 / KEYS : 1 << 30;    // blocks after which O is added to the sums
+    static __host__ __device__ constexpr int col_s(int u, int n) { return NQ == 2 ? u * 128 : (n & 1) * 128; }
+    static __host__ __device__ constexpr int col_o(int u) { return 256 + u * 128; }
+    static constexpr int COL_SUM = 384;
+    static constexpr int CHUNK = D == 64 ? 128 : 256;                  // bytes of a row that the epilogue stages at a time
+    static_assert(SOFT_WARPS * 32 * CHUNK <= Q_BYTES, "the epilogue stages rows where Q was");
     static_assert(STAGES >= 3, "a K and a V block in use and one on the way");
 };
 
@@ -85,11 +98,6 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     uint64_t d;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-__device__ __forceinline__ float max3_nan(float a, float b, float c) {       // NaN if any is
-    float d;
-    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -165,11 +173,11 @@ __device__ __forceinline__ void at_mma_ts(uint32_t d, uint32_t a, uint32_t b, ui
 __host__ __device__ constexpr uint32_t at_idesc(int n, bool bf, bool mn) {
     return (1u << 4) | (bf ? (1u << 7) | (1u << 10) : 0u) | (mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(AT_ROWS >> 4) << 24);
 }
-// sums = sums * by + O (first time: sums = O) for this thread's row, and O may be overwritten.
-template <int D>
+// sums = sums * by + O (first time: sums = O) for this thread's part of its row; O may then be overwritten.
+template <int D, int OUT>
 __device__ __forceinline__ void add_to_sums(uint32_t o_col, uint32_t sum_col, float *sums, bool live, bool more, float by) {
 #pragma unroll 1
-    for (int c = 0; c < D; c += 32) {
+    for (int c = 0; c < OUT; c += 32) {
         float o[32];
         at_ld32(o_col + c, o);
         if (D <= 128) {
@@ -200,52 +208,68 @@ __device__ __forceinline__ void add_to_sums(uint32_t o_col, uint32_t sum_col, fl
     }
 }
 
-// This thread's row of q (nothing: zeros) into shared memory as K-major operand tiles, one per term.  Returns the row's factor:
-// score -> q . k.
-template <int D, bool BF, int TERMS>
-__device__ __forceinline__ float load_q(const void *q, long long at, bool live, float sign, unsigned char *tile, int r) {
-    float factor = 1.0f, by = sign;
+// The barrier of the two warps that share 32 rows.
+__device__ __forceinline__ void pair_sync(int id) { asm volatile("barrier.cta.sync %0, 64;" ::"r"(id) : "memory"); }
+__device__ __forceinline__ bool pair_any(int id, bool v) {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %1, 0;\n\tbarrier.cta.red.or.pred p, %2, 64, q;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r) : "r"((uint32_t)v), "r"(id) : "memory");
+    return r != 0;
+}
+
+// Two values as two terms each: v = hi + lo.
+template <bool BF>
+__device__ __forceinline__ void split_two(float a, float b, uint32_t &hi, uint32_t &lo) {
+    hi = pack_half(a, b, BF);
+    const float2 h = unpack_half(hi, BF);
+    lo = pack_half(a - h.x, b - h.y, BF);
+}
+
+// This thread's row of q, or its half of it (nothing: zeros), into shared memory as K-major operand tiles, one per term: all its
+// loads first.  Returns the row's factor: score -> q . k.  told: where the threads of a row exchange the row's largest value.
+template <int D, bool BF, int TERMS, int SHARE>
+__device__ __forceinline__ float load_q(const void *q, long long at, bool live, float sign, unsigned char *tile, int r, int half, float *told, int mine,
+                                        int other, int pair_bar) {
+    constexpr int N = D / SHARE;
+    const int c0 = half * N;
+    float factor = 1.0f;
+    // elements c .. c + 7 of row r: slab c / 64, 16-byte piece (c % 64) / 8 swizzled by the row
+    auto place = [&](int c) { return tile + (c >> 6) * (AT_ROWS * 128) + r * 128 + ((((c & 63) >> 3) ^ (r & 7)) << 4); };
     if (TERMS == 2) {
-        const float *src = static_cast<const float *>(q) + at;
+        const float *src = static_cast<const float *>(q) + at + c0;
+        float4 v[N / 4];
+#pragma unroll
+        for (int i = 0; i < N / 4; i++) v[i] = live ? *reinterpret_cast<const float4 *>(src + 4 * i) : make_float4(0.f, 0.f, 0.f, 0.f);
         float top = 0.0f;
-        if (live) {
-#pragma unroll 16
-            for (int c = 0; c < D; c += 4) {
-                const float4 v = *reinterpret_cast<const float4 *>(src + c);
-                top = fmaxf(top, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
-            }
+#pragma unroll
+        for (int i = 0; i < N / 4; i++) top = fmaxf(top, fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)), fmaxf(fabsf(v[i].z), fabsf(v[i].w))));
+        if (SHARE == 2) {
+            told[mine] = top;
+            pair_sync(pair_bar);
+            top = fmaxf(top, told[other]);
         }
         const uint32_t ex = __float_as_uint(top) & 0x7f800000u;            // as in the kernel for few rows
-        if (ex > 0x01000000u && ex < 0x7e000000u) {
-            factor = __uint_as_float(ex);
-            by = sign * __uint_as_float(0x7f000000u - ex);
-        }
-    }
-#pragma unroll 8
-    for (int c = 0; c < D; c += 8) {
-        // elements c .. c + 7 of row r: slab c / 64, 16-byte piece (c % 64) / 8 swizzled by the row
-        unsigned char *to = tile + (c >> 6) * (AT_ROWS * 128) + r * 128 + ((((c & 63) >> 3) ^ (r & 7)) << 4);
-        uint32_t hi[4] = {0u, 0u, 0u, 0u}, lo[4] = {0u, 0u, 0u, 0u};
-        if (live) {
-            if (TERMS == 2) {
-                const float4 x = *reinterpret_cast<const float4 *>(static_cast<const float *>(q) + at + c);
-                const float4 y = *reinterpret_cast<const float4 *>(static_cast<const float *>(q) + at + c + 4);
-                const float v[8] = {x.x * by, x.y * by, x.z * by, x.w * by, y.x * by, y.y * by, y.z * by, y.w * by};
+        const bool scalable = ex > 0x01000000u && ex < 0x7e000000u;
+        const float by = scalable ? sign * __uint_as_float(0x7f000000u - ex) : sign;
+        factor = scalable ? __uint_as_float(ex) : 1.0f;
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    hi[e] = pack_half(v[2 * e], v[2 * e + 1], BF);
-                    const float2 h = unpack_half(hi[e], BF);
-                    lo[e] = pack_half(v[2 * e] - h.x, v[2 * e + 1] - h.y, BF);
-                }
-            } else {
-                const uint16_t *src = static_cast<const uint16_t *>(q) + at + c;   // rows start on 8 bytes
-                const uint2 x = *reinterpret_cast<const uint2 *>(src), y = *reinterpret_cast<const uint2 *>(src + 4);
-                const uint32_t flip = sign < 0.0f ? 0x80008000u : 0u;
-                hi[0] = x.x ^ flip; hi[1] = x.y ^ flip; hi[2] = y.x ^ flip; hi[3] = y.y ^ flip;
-            }
+        for (int i = 0; i < N / 8; i++) {
+            uint4 hi, lo;
+            split_two<BF>(v[2 * i].x * by, v[2 * i].y * by, hi.x, lo.x);
+            split_two<BF>(v[2 * i].z * by, v[2 * i].w * by, hi.y, lo.y);
+            split_two<BF>(v[2 * i + 1].x * by, v[2 * i + 1].y * by, hi.z, lo.z);
+            split_two<BF>(v[2 * i + 1].z * by, v[2 * i + 1].w * by, hi.w, lo.w);
+            *reinterpret_cast<uint4 *>(place(c0 + 8 * i)) = hi;
+            *reinterpret_cast<uint4 *>(place(c0 + 8 * i) + AT_ROWS * D * 2) = lo;
         }
-        *reinterpret_cast<uint4 *>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        if (TERMS == 2) *reinterpret_cast<uint4 *>(to + AT_ROWS * D * 2) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    } else {
+        const uint16_t *src = static_cast<const uint16_t *>(q) + at + c0;  // rows start on 8 bytes
+        uint2 v[N / 4];
+#pragma unroll
+        for (int i = 0; i < N / 4; i++) v[i] = live ? *reinterpret_cast<const uint2 *>(src + 4 * i) : make_uint2(0u, 0u);
+        const uint32_t flip = sign < 0.0f ? 0x80008000u : 0u;
+#pragma unroll
+        for (int i = 0; i < N / 8; i++)
+            *reinterpret_cast<uint4 *>(place(c0 + 8 * i)) = make_uint4(v[2 * i].x ^ flip, v[2 * i].y ^ flip, v[2 * i + 1].x ^ flip, v[2 * i + 1].y ^ flip);
     }
     return factor;
 }
@@ -259,9 +283,12 @@ __global__ void __launch_bounds__(AtShape<D, TERMS>::THREADS, 1) attn_tiles_kern
     unsigned char *smem = reinterpret_cast<unsigned char *>(((uintptr_t)at_raw + 1023) & ~(uintptr_t)1023);
     unsigned char *ring = smem + S::Q_BYTES;
     uint64_t *bars = reinterpret_cast<uint64_t *>(ring + STAGES * STAGE);
-    uint64_t *kv_full = bars, *kv_empty = bars + 8, *s_full = bars + 16, *p_full = bars + 18, *o_done = bars + 20, *q_full = bars + 22, *raw = bars + 24;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 26);
+    uint64_t *kv_full = bars, *kv_empty = kv_full + AT_MAX_STAGES, *s_full = kv_empty + AT_MAX_STAGES, *p_full = s_full + 2;
+    uint64_t *o_done = p_full + 2, *q_full = o_done + 2, *raw = q_full + 2;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(raw + 1);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    volatile int *told_stop = abort_flag + 2;                                                          // [warp]
+    float *told = reinterpret_cast<float *>(reinterpret_cast<unsigned char *>(bars) + 512);            // [half][row]
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, split = blockIdx.z;
     const int kv_heads = a.q_heads / a.group, kvh = blockIdx.x % kv_heads;
     unsigned *status = a.batch.status;
@@ -293,7 +320,8 @@ __global__ void __launch_bounds__(AtShape<D, TERMS>::THREADS, 1) attn_tiles_kern
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; s++) { mbar_init(&kv_full[s], 1); mbar_init(&kv_empty[s], 1); }
-        for (int u = 0; u < 2; u++) { mbar_init(&s_full[u], 1); mbar_init(&p_full[u], 4); mbar_init(&o_done[u], 1); mbar_init(&q_full[u], 4); }
+        for (int u = 0; u < 2; u++) { mbar_init(&s_full[u], 1); mbar_init(&q_full[u], 4 * S::SHARE); }
+        for (int u = 0; u < 2; u++) { mbar_init(&p_full[u], 4 * S::SHARE); mbar_init(&o_done[u], 1); }
         mbar_init(raw, 1);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -312,14 +340,16 @@ __global__ void __launch_bounds__(AtShape<D, TERMS>::THREADS, 1) attn_tiles_kern
     // Register split (NQ 2): 384 threads are launched with 168 registers each; 2 * 224 + 56 = 3 * 168.
     if (warp < S::SOFT_WARPS) {
         if (NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
-        // ---------------- softmax of tile u: thread = row
-        const int u = warp >> 2, quarter = warp & 3;
+        // ---------------- softmax of tile u.  Where two threads share a row, each takes half of a block's keys (and of the output's
+        // columns); both keep the same maximum, and agree on it and on giving up at the pair's barrier.
+        const int u = NQ == 2 ? warp >> 2 : 0, half = S::SHARE == 2 ? warp >> 2 : 0, quarter = warp & 3, pair_bar = 1 + quarter;
+        const int mine = half * AT_ROWS + quarter * 32 + lane, other = (1 - half) * AT_ROWS + quarter * 32 + lane;
         const int r0 = t.row0 + u * AT_ROWS, row = r0 + quarter * 32 + lane;
         const bool live = row < t.n_rows;
         unsigned char *q_tile = smem + u * TERMS * S::Q_TERM;
         const long long token = live ? t.token0 + row / a.group : 0;
         const int head = kvh * a.group + (live ? row % a.group : 0);
-        float factor = load_q<D, BF, TERMS>(a.q, token * a.q_stride + (long long)head * D, live, a.scale_log2 < 0.0f ? -1.0f : 1.0f, q_tile, quarter * 32 + lane);
+        float factor = load_q<D, BF, TERMS, S::SHARE>(a.q, token * a.q_stride + (long long)head * D, live, a.scale_log2 < 0.0f ? -1.0f : 1.0f, q_tile, quarter * 32 + lane, half, told, mine, other, pair_bar);
         factor = fminf(fmaxf(factor * fabsf(a.scale_log2), 1e-37f), 3e38f);  // a masked score (-inf) has to stay -inf when multiplied
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
@@ -327,129 +357,138 @@ __global__ void __launch_bounds__(AtShape<D, TERMS>::THREADS, 1) attn_tiles_kern
         int see_lo = 0, see_hi = 0;
         if (live) row_range(a, t, row, see_lo, see_hi);
         const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
-        const uint32_t o_col = lane_base + S::COL_O + u * S::O_STEP;
+        const uint32_t o_col = lane_base + S::col_o(u) + half * S::OUT;
         const long long slot = ((long long)split * a.batch.M + token) * a.q_heads + head;
         // dim 256: the sums of earlier blocks wait in the row's place in memory
-        float *sums = TERMS == 2 && D == 256 ? (alone ? static_cast<float *>(a.out) + token * a.out_stride + (long long)head * D : a.part_o + slot * D) : nullptr;
+        float *sums = TERMS == 2 && D == 256 ? (alone ? static_cast<float *>(a.out) + token * a.out_stride + (long long)head * D : a.part_o + slot * D) + half * S::OUT : nullptr;
         float m = live ? -INFINITY : 0.0f, l = 0.0f, m_sums = -INFINITY;   // (rows past the tile's last only keep out of the way)
         bool ok = true;
-        for (int blk = first[u], n = 0; blk < last[u]; blk++, n++) {
-            const int sb = NQ == 2 ? u : n & 1;
-            const uint32_t s_col = lane_base + S::COL_S + sb * 128;
-            if (!at_wait_warp(&s_full[sb], NQ == 2 ? (uint32_t)n & 1u : (uint32_t)(n >> 1) & 1u, abort_flag, status)) { ok = false; break; }
+        auto o_wait = [&](int n) {                           // the product of block n is in O
+            ok = ok && at_wait_warp(&o_done[u], (uint32_t)n & 1u, abort_flag, status);
             tc_fence_after();
-            float x[KEYS];
+            return ok;
+        };
+        for (int blk = first[u], n = 0; blk < last[u]; blk++, n++) {
+            const uint32_t s_col = lane_base + S::col_s(u, n) + half * S::COLS, p_col = lane_base + S::col_s(u, n) + half * (S::COLS / 2);
+            const int key0 = blk * KEYS + half * S::COLS;
+            ok = ok && (NQ == 2 ? at_wait_warp(&s_full[u], (uint32_t)n & 1u, abort_flag, status) : at_wait_warp(&s_full[n & 1], (uint32_t)(n >> 1) & 1u, abort_flag, status));
+            tc_fence_after();
+            float x[S::COLS];
 #pragma unroll
-            for (int c = 0; c < KEYS; c += 32) at_ld32(s_col + c, x + c);
+            for (int c = 0; c < S::COLS; c += 32) at_ld32(s_col + c, x + c);
             at_wait_ld();
-            const int key0 = blk * KEYS;
-            // Most blocks raise no row's maximum by more than the slack: their probabilities are formed against the maximum so far
-            // while the block's own is still being looked for, and only kept if it is within the slack (NaN is not).
-            const bool flush = TERMS == 2 && n > 0 && n % S::FLUSH == 0;
-            const bool edge = __any_sync(0xffffffffu, live && (key0 < see_lo || key0 + KEYS > see_hi));
-            bool done = false;
-            if (TERMS == 1 && !__any_sync(0xffffffffu, edge || (live && m == -INFINITY))) {
+            bool flushed = false;
+            if (TERMS == 2 && n > 0 && n % S::FLUSH == 0) {
+                o_wait(n - 1);
+                add_to_sums<D, S::OUT>(o_col, lane_base + S::COL_SUM + half * S::OUT, sums, live, n > S::FLUSH, m_sums == m ? 1.0f : exp2_fast(m_sums - m));
+                m_sums = m;
+                flushed = true;
+            }
+            // Most blocks raise no row's maximum by much: their probabilities are formed against the maximum so far, without looking
+            // for the block's own, and kept if their sum, and with it each of them, is in f16's range (NaN is not).
+            const bool edge = live && (blk * KEYS < see_lo || (blk + 1) * KEYS > see_hi);
+            bool again = __any_sync(0xffffffffu, !ok || edge || (live && m == -INFINITY));
+            float more = 0.0f, slack = AT_SLACK;
+            // The probabilities overwrite scores: not before the other thread of the row has read its own.
+            if (S::SHARE == 2) pair_sync(pair_bar);
+            if (!again) {
                 const uint64_t by = pair(factor, factor), less = pair(AT_SHIFT - m, AT_SHIFT - m);
                 uint64_t sum[2] = {0ull, 0ull};
-                float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int c = 0; c < KEYS; c += 32) {
-                    uint32_t p16[16];
+                for (int c = 0; c < S::COLS; c += 32) {
+                    uint32_t p16[16], lo16[16];
 #pragma unroll
                     for (int i = 0; i < 16; i++) {
                         const float x0 = x[c + 2 * i], x1 = x[c + 2 * i + 1];
                         const uint64_t y = fma2(pair(x0, x1), by, less);
                         float p0, p1;
-                        if (i % 8 < AT_POLY) {
+                        if (TERMS == 1 && i % 8 < AT_POLY) {
                             exp2_poly(y, p0, p1);
                         } else {
                             unpair(y, p0, p1);
                             p0 = exp2_fast(p0);
                             p1 = exp2_fast(p1);
                         }
-                        tops[i & 3] = max3_nan(tops[i & 3], x0, x1);
                         sum[i & 1] = add2(sum[i & 1], pair(p0, p1));
-                        p16[i] = pack_half(p0, p1, BF);
+                        if (TERMS == 2) split_two<BF>(p0, p1, p16[i], lo16[i]);
+                        else p16[i] = pack_half(p0, p1, BF);
                     }
-                    at_st16(s_col + c / 2, p16);
+                    at_st16(p_col + c / 2, p16);
+                    if (TERMS == 2) at_st16(p_col + KEYS / 2 + c / 2, lo16);
                 }
-                const float top = max3_nan(max3_nan(tops[0], tops[1], tops[2]), tops[3], tops[3]) * factor;
-                done = __all_sync(0xffffffffu, top <= m + AT_SLACK || !live);
-                if (done) {
-                    float s0, s1;
-                    unpair(add2(sum[0], sum[1]), s0, s1);
-                    l += s0 + s1;
+                float s0, s1;
+                unpair(add2(sum[0], sum[1]), s0, s1);
+                more = s0 + s1;
+                again = !__all_sync(0xffffffffu, more <= AT_SUM_MOST || !live);
+                slack = 0.0f;
+            }
+            if (S::SHARE == 2) again = pair_any(pair_bar, again);
+            if (again) {
+                at_wait_st();                                // what a failed attempt stored is stored again
+                if (edge) {
+                    const unsigned span = (unsigned)max(0, see_hi - see_lo);
+#pragma unroll
+                    for (int c = 0; c < S::COLS; c++)
+                        if ((unsigned)(key0 + c - see_lo) >= span) x[c] = -INFINITY;
                 }
-            }
-            if (!done) {
-            if (edge) {
-                const unsigned span = (unsigned)max(0, see_hi - see_lo);
+                float tops[4];                               // four chains: one would be COLS dependent steps
 #pragma unroll
-                for (int c = 0; c < KEYS; c++)
-                    if ((unsigned)(key0 + c - see_lo) >= span) x[c] = -INFINITY;
-            }
-            float tops[8];                                                   // eight chains: one would be 128 dependent steps
+                for (int c = 0; c < 4; c++) tops[c] = fmaxf(x[c], x[c + 4]);
 #pragma unroll
-            for (int c = 0; c < 8; c++) tops[c] = fmaxf(x[c], x[c + 8]);
+                for (int c = 8; c < S::COLS; c += 8)
 #pragma unroll
-            for (int c = 16; c < KEYS; c += 16)
-#pragma unroll
-                for (int e = 0; e < 8; e++) tops[e] = max3(tops[e], x[c + e], x[c + e + 8]);
-            const float top = max3(max3(tops[0], tops[1], tops[2]), max3(tops[3], tops[4], tops[5]), fmaxf(tops[6], tops[7])) * factor;
-            if (flush) {
-                if (!at_wait_warp(&o_done[0], (uint32_t)(n - 1) & 1u, abort_flag, status)) { ok = false; break; }
-                tc_fence_after();
-                add_to_sums<D>(lane_base + S::COL_O, lane_base + S::COL_SUM, sums, live, n > S::FLUSH, m_sums == m ? 1.0f : exp2_fast(m_sums - m));
-                m_sums = m;
-            }
-            const bool grow = top > m + AT_SLACK;
-            if (__any_sync(0xffffffffu, grow)) {
-                const float mn = grow ? top : m;
-                const float f = mn == m ? 1.0f : exp2_fast(m - mn);
-                m = mn;
-                l *= f;
-                if (n > 0 && !flush) {
-                    // the product of the block before has to be in O: with one score buffer its completion came before these
-                    // scores', with two it has a barrier of its own
-                    if (NQ == 1) {
-                        if (!at_wait_warp(&o_done[0], (uint32_t)(n - 1) & 1u, abort_flag, status)) { ok = false; break; }
-                        tc_fence_after();
-                    }
+                    for (int e = 0; e < 4; e++) tops[e] = max3(tops[e], x[c + e], x[c + e + 4]);
+                float top = max3(fmaxf(tops[0], tops[1]), tops[2], tops[3]) * factor;
+                if (S::SHARE == 2) {
+                    told[mine] = top;
+                    if (lane == 0) told_stop[warp] = !ok;
+                    pair_sync(pair_bar);
+                    top = fmaxf(top, told[other]);
+                    ok = (told_stop[warp] | told_stop[warp ^ 4]) == 0;
+                }
+                if (!ok) break;
+                const bool grow = top > m + slack;
+                if (__any_sync(0xffffffffu, grow)) {
+                    const float mn = grow ? top : m;
+                    const float f = mn == m ? 1.0f : exp2_fast(m - mn);
+                    m = mn;
+                    l *= f;
+                    if (n > 0 && !flushed) {
+                        // (without AHEAD the product of the block before came ahead of these scores)
+                        if (S::AHEAD) o_wait(n - 1);
 #pragma unroll 1
-                    for (int c = 0; c < D; c += 32) {
-                        float o[32];
-                        at_ld32(o_col + c, o);
-                        at_wait_ld();
+                        for (int c = 0; c < S::OUT; c += 32) {
+                            float o[32];
+                            at_ld32(o_col + c, o);
+                            at_wait_ld();
 #pragma unroll
-                        for (int i = 0; i < 32; i++) o[i] *= f;
-                        at_st32f(o_col + c, o);
+                            for (int i = 0; i < 32; i++) o[i] *= f;
+                            at_st32f(o_col + c, o);
+                        }
                     }
                 }
-            }
-            const float off = m == -INFINITY ? 0.0f : m - AT_SHIFT;
-            float part[4] = {0.f, 0.f, 0.f, 0.f};
+                const float off = m == -INFINITY ? 0.0f : m - AT_SHIFT;
+                float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int c = 0; c < KEYS; c += 32) {
-                uint32_t hi16[16], lo16[16];
+                for (int c = 0; c < S::COLS; c += 32) {
+                    uint32_t hi16[16], lo16[16];
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const float p0 = exp2_fast(fmaf(x[c + 2 * i], factor, -off)), p1 = exp2_fast(fmaf(x[c + 2 * i + 1], factor, -off));
-                    part[i & 3] += p0 + p1;
-                    hi16[i] = pack_half(p0, p1, BF);
-                    if (TERMS == 2) {
-                        const float2 h = unpack_half(hi16[i], BF);
-                        lo16[i] = pack_half(p0 - h.x, p1 - h.y, BF);
+                    for (int i = 0; i < 16; i++) {
+                        const float p0 = exp2_fast(fmaf(x[c + 2 * i], factor, -off)), p1 = exp2_fast(fmaf(x[c + 2 * i + 1], factor, -off));
+                        part[i & 3] += p0 + p1;
+                        if (TERMS == 2) split_two<BF>(p0, p1, hi16[i], lo16[i]);
+                        else hi16[i] = pack_half(p0, p1, BF);
                     }
+                    at_st16(p_col + c / 2, hi16);
+                    if (TERMS == 2) at_st16(p_col + KEYS / 2 + c / 2, lo16);
                 }
-                at_st16(s_col + c / 2, hi16);
-                if (TERMS == 2) at_st16(s_col + KEYS / 2 + c / 2, lo16);
+                more = (part[0] + part[1]) + (part[2] + part[3]);
             }
-            l += (part[0] + part[1]) + (part[2] + part[3]);
-            }
+            l += more;
             at_wait_st();
-            // With two score buffers the scores run a block ahead: passing these probabilities on only when the product before has
-            // ended keeps every waiter within one phase of its barrier (a parity cannot tell a phase from the one two before).
-            if (NQ == 1 && n > 0 && !at_wait_warp(&o_done[0], (uint32_t)(n - 1) & 1u, abort_flag, status)) { ok = false; break; }
+            // With the scores a block ahead, passing these probabilities on only when the product before has ended keeps every waiter
+            // within one phase of its barrier (a parity cannot tell a phase from the one two before).
+            if (S::AHEAD && n > 0) o_wait(n - 1);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&p_full[u]);
@@ -457,51 +496,95 @@ __global__ void __launch_bounds__(AtShape<D, TERMS>::THREADS, 1) attn_tiles_kern
         // ---------------- the tile's rows: O / l to out, or O and (m, l) to the split's place
         const int blocks = last[u] - first[u];
         if (ok && blocks > 0) {
-            ok = at_wait_warp(&o_done[u], NQ == 2 ? 0u : (uint32_t)(blocks - 1) & 1u, abort_flag, status);
-            tc_fence_after();
+            if (S::AHEAD) o_wait(blocks - 1);
+            else {
+                ok = at_wait_warp(&o_done[u], 0u, abort_flag, status);
+                tc_fence_after();
+            }
+        }
+        if (S::SHARE == 2) {
+            pair_sync(pair_bar);
+            told[mine] = l;
+            pair_sync(pair_bar);
+            l += told[other];
         }
         if (ok) {
             const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f, sums_by = m_sums == m ? 1.0f : exp2_fast(m_sums - m);
-            if (live && !alone) a.part_ml[slot] = make_float2(m, l);
-            if (live && alone && a.part_ml) a.part_ml[token * a.q_heads + head] = make_float2(0.0f, -1.0f);
+            if (live && half == 0 && !alone) a.part_ml[slot] = make_float2(m, l);
+            if (live && half == 0 && alone && a.part_ml) a.part_ml[token * a.q_heads + head] = make_float2(0.0f, -1.0f);
             if (alone || blk1 > blk0) {
+                // Rows leave through the tile's part of Q's shared memory (its MMAs have ended), S::CHUNK bytes of each at a time, so
+                // that a warp writes whole stretches of a row instead of one piece of 32 rows.
+                const int es = alone && a.act_type != OJAS_B200_F32 ? 2 : 4, per = S::CHUNK / es;      // element size, columns of a chunk
+                unsigned char *stage = smem + warp * (S::CHUNK * 32);
+                unsigned char *to = alone ? static_cast<unsigned char *>(a.out) + (token * a.out_stride + (long long)head * D + half * S::OUT) * es
+                                          : reinterpret_cast<unsigned char *>(a.part_o + slot * D + half * S::OUT);
+                if (!live) to = nullptr;
+                if (blocks == 0) asm volatile("barrier.cta.sync %0, %1;" ::"r"(9 + u), "n"(128 * S::SHARE) : "memory");   // no MMA has waited for all of Q here
+                const float by = alone ? inv : 1.0f;
+                const bool wide = !alone || a.out_stride * es % 16 == 0;
+                constexpr int PIECES = S::CHUNK / 16;        // 16-byte pieces of a row's chunk; piece p of row r lies at p ^ (r % 8)
 #pragma unroll 1
-                for (int c = 0; c < D; c += 32) {
-                    float o[32];
-                    if (blocks > 0) {
-                        at_ld32(o_col + c, o);
-                        if (TERMS == 2 && blocks > S::FLUSH) {
-                            float e[32];
-                            if (D <= 128) at_ld32(lane_base + S::COL_SUM + c, e);
-                            at_wait_ld();
-                            if (D > 128) {
+                for (int c0 = 0; c0 < S::OUT; c0 += per) {
+#pragma unroll 1
+                    for (int c = c0; c < c0 + per; c += 32) {
+                        float o[32];
+                        if (blocks > 0) {
+                            at_ld32(o_col + c, o);
+                            if (TERMS == 2 && blocks > S::FLUSH) {
+                                float e[32];
+                                if (D <= 128) at_ld32(lane_base + S::COL_SUM + half * S::OUT + c, e);
+                                at_wait_ld();
+                                if (D > 128) {
 #pragma unroll
-                                for (int i = 0; i < 32; i++) e[i] = live ? sums[c + i] : 0.0f;
+                                    for (int i = 0; i < 32; i++) e[i] = live ? sums[c + i] : 0.0f;
+                                }
+#pragma unroll
+                                for (int i = 0; i < 32; i++) o[i] = fmaf(e[i], sums_by, o[i]);
                             }
+                            at_wait_ld();
+                        } else {
 #pragma unroll
-                            for (int i = 0; i < 32; i++) o[i] = fmaf(e[i], sums_by, o[i]);
+                            for (int i = 0; i < 32; i++) o[i] = 0.0f;
                         }
-                        at_wait_ld();
-                    } else {
+                        unsigned char *row_at = stage + lane * S::CHUNK;
+                        const int p0 = (c - c0) * es / 16;
+                        if (es == 4) {
 #pragma unroll
-                        for (int i = 0; i < 32; i++) o[i] = 0.0f;
+                            for (int i = 0; i < 8; i++)
+                                *reinterpret_cast<float4 *>(row_at + (((p0 + i) ^ (lane & 7)) << 4)) = make_float4(o[4 * i] * by, o[4 * i + 1] * by, o[4 * i + 2] * by, o[4 * i + 3] * by);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 4; i++)
+                                *reinterpret_cast<uint4 *>(row_at + (((p0 + i) ^ (lane & 7)) << 4)) =
+                                    make_uint4(pack_half(o[8 * i] * by, o[8 * i + 1] * by, BF), pack_half(o[8 * i + 2] * by, o[8 * i + 3] * by, BF),
+                                               pack_half(o[8 * i + 4] * by, o[8 * i + 5] * by, BF), pack_half(o[8 * i + 6] * by, o[8 * i + 7] * by, BF));
+                        }
                     }
                     __syncwarp();
-                    const long long at = alone ? token * a.out_stride + (long long)head * D + c : slot * D + c;
-#pragma unroll
-                    for (int i = 0; i < 32; i += 4) {
-                        const float4 v = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-                        if (!live) { }
-                        else if (alone) store_elem4(a.out, a.act_type, at + i, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
-                        else *reinterpret_cast<float4 *>(a.part_o + at + i) = v;
+#pragma unroll 4
+                    for (int i = 0; i < PIECES; i++) {
+                        const int r = (i * 32 + lane) / PIECES, p = lane % PIECES;
+                        unsigned char *row_to = reinterpret_cast<unsigned char *>(__shfl_sync(0xffffffffu, (unsigned long long)to, r));
+                        const uint4 v = *reinterpret_cast<const uint4 *>(stage + r * S::CHUNK + ((p ^ (r & 7)) << 4));
+                        if (row_to) {
+                            uint4 *dst = reinterpret_cast<uint4 *>(row_to + c0 * es + p * 16);
+                            if (wide) *dst = v;
+                            else {                           // 16-bit rows that start on 8 bytes
+                                reinterpret_cast<uint2 *>(dst)[0] = make_uint2(v.x, v.y);
+                                reinterpret_cast<uint2 *>(dst)[1] = make_uint2(v.z, v.w);
+                            }
+                        }
                     }
+                    __syncwarp();
                 }
             }
         }
     } else {
     if (NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == S::SOFT_WARPS) {
-        // ---------------- MMA issue: the warp waits together, one elected lane issues.  Ring order: see the loader
+        // ---------------- MMA issue: the warp waits together, one elected lane issues (one warp for both tiles: with one each their
+        // MMAs mix, and both tiles wait longer for theirs).  Ring order: see the loader.
         constexpr uint32_t ID_S = at_idesc(KEYS, BF, false), ID_O = at_idesc(D, BF, true);
         bool ok = true;
         const int b0 = __shfl_sync(0xffffffffu, blk0, 0), b1 = __shfl_sync(0xffffffffu, blk1, 0);
@@ -514,96 +597,92 @@ __global__ void __launch_bounds__(AtShape<D, TERMS>::THREADS, 1) attn_tiles_kern
         const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
         auto next = [&]() { if (++s == STAGES) { s = 0; phase ^= 1u; } };
         auto wait = [&](uint64_t *bar, uint32_t parity) { ok = ok && at_wait_warp(bar, parity, abort_flag, status); };
-        auto scores = [&](int u, int buf, int stage) {
+        auto scores = [&](int u, int n, int stage) {
             const uint32_t kd = at_desc(ring_at + stage * STAGE, 16);
 #pragma unroll
             for (int term = 0; term < TERMS; term++) {     // the low term first, while the sums are small
                 const uint32_t qd = at_desc(q_at + (u * TERMS + TERMS - 1 - term) * S::Q_TERM, 16);
 #pragma unroll
                 for (int k = 0; k < D / 16; k++)           // 16 of dim: 32 bytes of a row, four per slab
-                    at_mma_ss(tm + S::COL_S + buf * 128, qd + (k >> 2) * (AT_ROWS * 128 / 16) + (k & 3) * 2, kd + (k >> 2) * (KEYS * 128 / 16) + (k & 3) * 2, ID_S,
+                    at_mma_ss(tm + S::col_s(u, n), qd + (k >> 2) * (AT_ROWS * 128 / 16) + (k & 3) * 2, kd + (k >> 2) * (KEYS * 128 / 16) + (k & 3) * 2, ID_S,
                               term + k > 0);
             }
-            umma_commit(&s_full[buf]);
+            umma_commit(&s_full[NQ == 2 ? u : n & 1]);
         };
-        auto values = [&](int u, int buf, int stage, bool begin) {
+        auto values = [&](int u, int n, int stage, bool last_block) {
             const uint32_t vd = at_desc(ring_at + stage * STAGE, KEYS * 128);
 #pragma unroll
             for (int term = 0; term < TERMS; term++)
 #pragma unroll
                 for (int k = 0; k < KEYS / 16; k++)        // 16 keys: 8 columns of packed P, 2048 bytes of V
-                    at_mma_ts(tm + S::COL_O + u * S::O_STEP, tm + S::COL_S + buf * 128 + term * (KEYS / 2) + k * 8, vd + k * (2048 / 16), ID_O, !begin || term + k > 0);
+                    at_mma_ts(tm + S::col_o(u), tm + S::col_s(u, n) + term * (KEYS / 2) + k * 8, vd + k * (2048 / 16), ID_O, n % S::FLUSH != 0 || term + k > 0);
+            if (S::AHEAD || last_block) umma_commit(&o_done[u]);
         };
         for (int u = 0; u < NQ; u++)
             if (to[u] > from[u]) wait(&q_full[u], 0);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        if (NQ == 2) {
-            int v_stage = 0, n[2] = {0, 0};
-            for (int i = b0; ok && i <= b1; i++) {
-                // block i's K is at the ring's head, block i - 1's V one behind it: (K0) (V0 K1) (V1 K2) ... (Vlast)
-                if (i > b0) { wait(&kv_full[s], phase); v_stage = s; next(); }
-                const int k_stage = s;
-                const uint32_t k_phase = phase;
-                if (i < b1) next();
-#pragma unroll
-                for (int u = 0; u < NQ; u++) {
-                    const bool has_v = i - 1 >= from[u] && i - 1 < to[u], has_k = i >= from[u] && i < to[u];
-                    if (has_v) {
-                        wait(&p_full[u], (uint32_t)n[u] & 1u);
-                        if (!ok) break;
-                        tc_fence_after();
-                    }
-                    if (elect_one()) {
-                        if (has_v) {
-                            values(u, u, v_stage, n[u] == 0);
-                            if (i == to[u]) umma_commit(&o_done[u]);
-                        }
-                        if (u == NQ - 1 && i > b0) umma_commit(&kv_empty[v_stage]);
-                    }
-                    __syncwarp();
-                    if (u == 0 && i < b1) wait(&kv_full[k_stage], k_phase);
-                    if (!ok) break;
-                    tc_fence_after();
-                    if (elect_one()) {
-                        if (has_k) scores(u, u, k_stage);
-                        if (u == NQ - 1 && i < b1) umma_commit(&kv_empty[k_stage]);
-                    }
-                    __syncwarp();
-                    n[u] += has_v;
-                }
-            }
-        } else {
-            for (int i = b0; ok && i <= b1; i++) {
-                // (K0) (K1 V0) (K2 V1) ... (Vlast)
+        int n_s[NQ] = {}, n_o[NQ] = {};                      // blocks of a tile whose scores, whose products have been issued
+        for (int i = b0; ok && i <= b1; i++) {
+            if (S::AHEAD) {
+                // (K0) (K1 V0) (K2 V1) ... (Vlast): block i's scores, then the products of block i - 1
                 if (i < b1) {
                     wait(&kv_full[s], phase);
                     if (!ok) break;
                     tc_fence_after();
                     if (elect_one()) {
-                        scores(0, (i - b0) & 1, s);
+                        scores(0, n_s[0], s);
                         umma_commit(&kv_empty[s]);
                     }
                     __syncwarp();
+                    n_s[0]++;
                     next();
                 }
                 if (i > b0) {
-                    const int n = i - 1 - b0;
                     wait(&kv_full[s], phase);
-                    wait(&p_full[0], (uint32_t)n & 1u);
+                    wait(&p_full[0], (uint32_t)n_o[0] & 1u);
                     if (!ok) break;
                     tc_fence_after();
                     if (elect_one()) {
-                        values(0, n & 1, s, n % S::FLUSH == 0);
-                        umma_commit(&o_done[0]);
+                        values(0, n_o[0], s, i == to[0]);
                         umma_commit(&kv_empty[s]);
                     }
                     __syncwarp();
+                    n_o[0]++;
                     next();
+                }
+            } else {
+                // (K0) (V0 K1) (V1 K2) ... (Vlast): a tile's products, then its next scores over the probabilities they read
+                const int v_stage = s;
+                if (i > b0) { wait(&kv_full[s], phase); next(); }
+                const int k_stage = s;
+                const uint32_t k_phase = phase;
+                if (i < b1) next();
+#pragma unroll
+                for (int u = 0; u < NQ; u++) {
+                    const bool has_o = i - 1 >= from[u] && i - 1 < to[u], has_s = i >= from[u] && i < to[u];
+                    if (has_o) wait(&p_full[u], (uint32_t)n_o[u] & 1u);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (elect_one()) {
+                        if (has_o) values(u, n_o[u], v_stage, i == to[u]);
+                        if (u == NQ - 1 && i > b0) umma_commit(&kv_empty[v_stage]);
+                    }
+                    __syncwarp();
+                    n_o[u] += has_o;
+                    if (u == 0 && i < b1) wait(&kv_full[k_stage], k_phase);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (elect_one()) {
+                        if (has_s) scores(u, n_s[u], k_stage);
+                        if (u == NQ - 1 && i < b1) umma_commit(&kv_empty[k_stage]);
+                    }
+                    __syncwarp();
+                    n_s[u] += has_s;
                 }
             }
         }
     } else if (warp == S::SOFT_WARPS + 1) {
-        // ---------------- loader: lane = one box (64 values x box_rows tokens).  NQ 2: K0 V0 K1 V1 ...; NQ 1: K0 K1 V0 K2 V1 ...
+        // ---------------- loader: lane = one box (64 values x box_rows tokens); K0 K1 V0 K2 V1 ... Vlast, or (not AHEAD) K0 V0 K1 V1 ...
         const int per_slab = KEYS / box_rows, part = lane % per_slab, slab = lane / per_slab;
         const bool has_box = slab < D / 64;
         const int *table = a.batch.table + (long long)t.seq * a.batch.table_stride;
@@ -655,11 +734,11 @@ __global__ void __launch_bounds__(AtShape<D, TERMS>::THREADS, 1) attn_tiles_kern
             advance();
             if (blk + 1 < blk1) next_page = look_up();
             copy(&map_k, false, blk, want, page, at);
-            if (NQ == 2) copy(&map_v, true, blk, want, page, at);
+            if (!S::AHEAD) copy(&map_v, true, blk, want, page, at);
             else if (blk > blk0) copy(&map_v, true, blk - 1, v_want, v_page, v_slot);
             v_want = want; v_page = page; v_slot = at;
         }
-        if (NQ == 1 && blk1 > blk0) copy(&map_v, true, blk1 - 1, v_want, v_page, v_slot);
+        if (S::AHEAD && blk1 > blk0) copy(&map_v, true, blk1 - 1, v_want, v_page, v_slot);
     }
     }
 
