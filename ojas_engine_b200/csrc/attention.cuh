@@ -85,7 +85,8 @@ __device__ __forceinline__ float exp2_fast(float x) {
 // What the planner decides for a call (attention.cu).
 struct AttnPlan {
     bool tensor;                         // the tcgen05 kernel
-    int rows, mt;                        // rows of a tile; 8-row MMA tiles per warp of the small kernel
+    bool two, cluster;                   // the kernel for few rows: two terms per value; the splits are a cluster
+    int rows, mt;                        // rows of a tile; MMA tiles per warp of the kernel for few rows
     long long tiles;                     // upper bound on the call's row tiles
     int splits, split_blocks, block;     // keys per block
     size_t workspace;
