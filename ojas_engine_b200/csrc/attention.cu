@@ -532,7 +532,8 @@ extern "C" size_t ojas_b200_attention_workspace_bytes(ojas_b200_ctx *ctx, const 
 
 template <int D, bool BF, bool TWO, int MT>
 static cudaError_t launch_rows(const ojas_b200_ctx *ctx, const ojas_b200_kv *kv, const AttnArgs &a, const AttnPlan &p) {
-    const cudaError_t e = cudaFuncSetAttribute(attn_rows_kernel<D, BF, TWO, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, ar_smem(D));
+    static std::atomic<uint64_t> ready{0};
+    const cudaError_t e = smem_once(ready, ctx->device, attn_rows_kernel<D, BF, TWO, MT>, ar_smem(D));
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)p.tiles, (unsigned)kv->heads, (unsigned)p.splits);

@@ -1,5 +1,7 @@
 // Attention over a paged cache: what its two kernels, the joining kernel and the entry point share.
 #pragma once
+#include <atomic>
+
 #include "attn.cuh"
 #include "tc_util.cuh"
 
@@ -80,6 +82,16 @@ __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// Allows a kernel its dynamic shared memory, once per device (a bit each; devices from 64 on are asked every time).
+template <typename K>
+static cudaError_t smem_once(std::atomic<uint64_t> &ready, int device, K kernel, int bytes) {
+    const uint64_t bit = device < 64 ? 1ull << device : 0ull;
+    if (bit && (ready.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) ready.fetch_or(bit, std::memory_order_relaxed);
+    return e;
 }
 
 // What the planner decides for a call (attention.cu).

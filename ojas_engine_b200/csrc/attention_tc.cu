@@ -208,6 +208,9 @@ __device__ __forceinline__ void add_to_sums(uint32_t o_col, uint32_t sum_col, fl
     }
 }
 
+// The lowest n bits (n below 0: none, above 32: all).
+__device__ __forceinline__ uint32_t below(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
+
 // The barrier of the two warps that share 32 rows.
 __device__ __forceinline__ void pair_sync(int id) { asm volatile("barrier.cta.sync %0, 64;" ::"r"(id) : "memory"); }
 __device__ __forceinline__ bool pair_any(int id, bool v) {
@@ -426,10 +429,12 @@ __global__ void __launch_bounds__(AtShape<D, TERMS>::THREADS, 1) attn_tiles_kern
             if (again) {
                 at_wait_st();                                // what a failed attempt stored is stored again
                 if (edge) {
-                    const unsigned span = (unsigned)max(0, see_hi - see_lo);
 #pragma unroll
-                    for (int c = 0; c < S::COLS; c++)
-                        if ((unsigned)(key0 + c - see_lo) >= span) x[c] = -INFINITY;
+                    for (int c = 0; c < S::COLS; c += 32) {  // a bit for each of 32 keys that the row sees
+                        const uint32_t seen = below(see_hi - key0 - c) & ~below(see_lo - key0 - c);
+#pragma unroll
+                        for (int i = 0; i < 32; i++) x[c + i] = seen >> i & 1u ? x[c + i] : -INFINITY;
+                    }
                 }
                 float tops[4];                               // four chains: one would be COLS dependent steps
 #pragma unroll
@@ -758,7 +763,8 @@ __global__ void __launch_bounds__(AtShape<D, TERMS>::THREADS, 1) attn_tiles_kern
 template <int D, bool BF, int TERMS>
 cudaError_t launch_tiles(const ojas_b200_ctx *ctx, const ojas_b200_kv *kv, const AttnArgs &a, const AttnPlan &p) {
     using S = AtShape<D, TERMS>;
-    cudaError_t e = cudaFuncSetAttribute(attn_tiles_kernel<D, BF, TERMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+    static std::atomic<uint64_t> ready{0};
+    const cudaError_t e = smem_once(ready, ctx->device, attn_tiles_kernel<D, BF, TERMS>, S::SMEM);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(p.tiles * (long long)kv->heads), 1, (unsigned)p.splits);

@@ -177,20 +177,18 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const AppendArgs a) {
     const int ux = threadIdx.x % turning, uy = threadIdx.x / turning, ny = blockDim.x / turning;   // (dim <= 256: at most 128 units)
     if (uy >= ny) return;
     const RopeUnit<VEC> unit(ux, rot, a.dim, a.interleaved), plain(ux, 0, a.dim, false);
-    const int rows = a.q_heads + 2 * a.kv_heads;
-    for (int r = uy; r < tokens * rows; r += ny) {
-        const int t = r / rows, h = r - t * rows;
+    for (int t = 0; t < tokens; t++) {
         if (!row_live[t]) continue;
         const long long tok = t0 + t;
         const float2 *cs = append_cs + t * half;
-        if (h < a.q_heads) {
-            unit.apply(a.q, a.x_type, tok * a.q_stride + (long long)h * a.dim, a.q_out, a.q_type, tok * a.q_out_stride + (long long)h * a.dim, cs);
-        } else if (row_at[t] >= 0) {
-            const bool is_k = h < a.q_heads + a.kv_heads;
-            const int kh = h - a.q_heads - (is_k ? 0 : a.kv_heads);
-            const long long to = row_at[t] + (long long)kh * a.head_stride;
-            if (is_k) unit.apply(a.k, a.x_type, tok * a.k_stride + (long long)kh * a.dim, a.kc, a.c_type, to, cs);
-            else plain.apply(a.v, a.x_type, tok * a.v_stride + (long long)kh * a.dim, a.vc, a.c_type, to, cs);
+#pragma unroll 4
+        for (int h = uy; h < a.q_heads; h += ny)
+            unit.apply(a.q, a.x_type, tok * a.q_stride + h * a.dim, a.q_out, a.q_type, tok * a.q_out_stride + h * a.dim, cs);
+        if (row_at[t] < 0) continue;
+        for (int h = uy; h < a.kv_heads; h += ny) {
+            const long long to = row_at[t] + (long long)h * a.head_stride;
+            unit.apply(a.k, a.x_type, tok * a.k_stride + h * a.dim, a.kc, a.c_type, to, cs);
+            plain.apply(a.v, a.x_type, tok * a.v_stride + h * a.dim, a.vc, a.c_type, to, cs);
         }
     }
 }

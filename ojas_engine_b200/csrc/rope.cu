@@ -111,10 +111,10 @@ __global__ void __launch_bounds__(256) rope_rows_kernel(const RopeArgs a) {
     const int units = rope_units(VEC, a.rot, a.dim);
     for (int u = threadIdx.x; u < units; u += blockDim.x) {
         const RopeUnit<VEC> unit(u, a.rot, a.dim, a.interleaved);
-        for (int r = threadIdx.y; r < tokens * a.heads; r += blockDim.y) {
-            const int t = r / a.heads, h = r - t * a.heads;
-            const long long xo = (t0 + t) * a.x_stride + (long long)h * a.dim, yo = (t0 + t) * a.y_stride + (long long)h * a.dim;
-            unit.apply(a.x, a.x_type, xo, a.y, a.y_type, yo, rope_cs + t * half);
+        for (int t = 0; t < tokens; t++) {
+            const long long xo = (t0 + t) * a.x_stride, yo = (t0 + t) * a.y_stride;
+#pragma unroll 4
+            for (int h = threadIdx.y; h < a.heads; h += blockDim.y) unit.apply(a.x, a.x_type, xo + h * a.dim, a.y, a.y_type, yo + h * a.dim, rope_cs + t * half);
         }
     }
 }

@@ -302,12 +302,16 @@ class B200Gpu:
         """Attention of the call's rows over their sequences' keys (scale: 1 / sqrt(dim) unless given).  Without a caller
         workspace a grow-only scratch buffer owned by this object is used; a buffer it outgrew stays allocated, because a
         captured graph may still use it."""
-        need = self._l.ojas_b200_attention_workspace_bytes(self._ctx, kv._h, seqs._ref, act_type, m, q_heads, window)
-        if workspace is None and need:
-            workspace = self._attn_ws[-1] if self._attn_ws else None
-            if workspace is None or workspace.nbytes < need:
-                workspace = self.alloc_bytes(max(need, 2 * workspace.nbytes if workspace else 0))
-                self._attn_ws.append(workspace)
+        if workspace is None:
+            shape = (kv.heads, kv.dim, kv.page_size, kv.type, act_type, m, q_heads, window, self._ctx.value)
+            need = seqs._need.get(shape)
+            if need is None:                       # depends on the bounds and counts alone, which a Seqs does not change
+                need = seqs._need[shape] = self.attention_workspace_bytes(kv, seqs, m, q_heads, act_type, window)
+            if need:
+                workspace = self._attn_ws[-1] if self._attn_ws else None
+                if workspace is None or workspace.nbytes < need:
+                    workspace = self.alloc_bytes(max(need, 2 * workspace.nbytes if workspace else 0))
+                    self._attn_ws.append(workspace)
         self._ck(self._l.ojas_b200_attention(self._ctx, kv._h, seqs._ref, act_type, q.ptr, q_stride, q_heads, kv.dim ** -0.5 if scale is None else scale,
                                              1 if causal else 0, window, out.ptr, out_stride, m, workspace.ptr if workspace else None,
                                              workspace.nbytes if workspace else 0))
@@ -465,6 +469,7 @@ class Seqs:
         self.cu, self.lens, self.table = cu, lens, table
         self._struct = _lib.SeqsStruct(cu.ptr, lens.ptr, table.ptr, n_seqs, table_stride, max_rows, max_len)
         self._ref = C.byref(self._struct)
+        self._need: dict = {}
 
 
 class ExpertCache:
