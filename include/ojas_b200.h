@@ -285,7 +285,8 @@ enum { OJAS_B200_ROPE_HALF = 0, OJAS_B200_ROPE_INTERLEAVED = 1 };
  *                  frequency for r_i >= beta_fast, has it divided by factor for r_i <= beta_slow, and is mixed linearly in
  *                  r_i between.
  * Rotated values are multiplied by magnitude.  create allocates rot_dim / 2 words on the device and copies them there (it
- * waits for the copy: set-up only); destroy frees them, after the launches that use them have ended. */
+ * waits for the copy: set-up only); destroy frees them (after the launches that use them have ended).  A rotation serves
+ * every context of its device and may outlive the one it was made with. */
 typedef struct ojas_b200_rope ojas_b200_rope;
 typedef struct {
     double factor, beta_fast, beta_slow;

@@ -305,6 +305,7 @@ __global__ void __launch_bounds__(AR_THREADS, MT == 2 || D == 256 ? 1 : 2) attn_
         for (int r = 0; r < R; r++) {
             l[i][r] += __shfl_xor_sync(0xffffffffu, l[i][r], 1);
             l[i][r] += __shfl_xor_sync(0xffffffffu, l[i][r], 2);
+            if (l[i][r] != l[i][r] && m[i][r] == -INFINITY) m[i][r] = 0.0f;       // nothing but NaN was seen: that is not "no key"
             if (q4 == 0) stats[warp * ROWS + i * 8 * R + r * 8 + g] = make_float2(m[i][r], l[i][r]);
         }
     }
@@ -570,7 +571,7 @@ extern "C" int ojas_b200_attention(ojas_b200_ctx *ctx, const ojas_b200_kv *kv, c
                                    size_t workspace_bytes) {
     if (!ctx) return OJAS_B200_E_ARG;
     if (!kv) return ojas_fail(ctx, OJAS_B200_E_ARG, "attention: null cache");
-    if (kv->ctx->device != ctx->device) return ojas_fail(ctx, OJAS_B200_E_ARG, "attention: the cache lives on device %d, the context on %d", kv->ctx->device, ctx->device);
+    if (kv->device != ctx->device) return ojas_fail(ctx, OJAS_B200_E_ARG, "attention: the cache lives on device %d, the context on %d", kv->device, ctx->device);
     char why[256];
     const int rc = ojas_b200_attention_check(kv->type, kv->page_size, kv->heads, kv->dim, act_type, q_heads, q, q_stride, out, out_stride, scale, causal, window, seqs, M, why, sizeof why);
     if (rc) return ojas_fail(ctx, rc, "%s", why);

@@ -515,7 +515,7 @@ __global__ void __launch_bounds__(AtShape<D, TERMS>::THREADS, 1) attn_tiles_kern
         }
         if (ok) {
             const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f, sums_by = m_sums == m ? 1.0f : exp2_fast(m_sums - m);
-            if (live && half == 0 && !alone) a.part_ml[slot] = make_float2(m, l);
+            if (live && half == 0 && !alone) a.part_ml[slot] = make_float2(l != l && m == -INFINITY ? 0.0f : m, l);   // (nothing but NaN seen is not "no key")
             if (live && half == 0 && alone && a.part_ml) a.part_ml[token * a.q_heads + head] = make_float2(0.0f, -1.0f);
             if (alone || blk1 > blk0) {
                 // Rows leave through the tile's part of Q's shared memory (its MMAs have ended), S::CHUNK bytes of each at a time, so

@@ -13,14 +13,14 @@ constexpr unsigned OJAS_ST_ATTN_WAIT = 0x200000u;  // a bounded wait of an atten
 // Rotation of one pair per frequency.  turns[i] is the frequency in turns per position as a 64-bit binary fraction, so
 // pos * turns[i] modulo 2^64 is the pair's angle modulo one turn, exactly, for every 32-bit position.
 struct ojas_b200_rope {
-    ojas_b200_ctx *ctx;
+    int device;
     uint32_t rot_dim;
     float magnitude;
     uint64_t *turns;          // device, rot_dim / 2
 };
 
 struct ojas_b200_kv {
-    ojas_b200_ctx *ctx;
+    int device;
     uint32_t type;            // OJAS_B200_F16 or OJAS_B200_BF16
     void *k, *v;
     size_t pages, page_size, heads, dim;

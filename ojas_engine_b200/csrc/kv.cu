@@ -67,7 +67,7 @@ extern "C" int ojas_b200_kv_create(ojas_b200_ctx *ctx, uint32_t type, void *k, v
     if (rc) return rc;
     ojas_b200_kv *c = new (std::nothrow) ojas_b200_kv();
     if (!c) return ojas_fail(ctx, OJAS_B200_E_LIMIT, "kv_create: out of host memory");
-    c->ctx = ctx; c->type = type; c->k = k; c->v = v;
+    c->device = ctx->device; c->type = type; c->k = k; c->v = v;
     c->pages = pages; c->page_size = page_size; c->heads = heads; c->dim = dim;
     c->page_stride = page_stride; c->head_stride = head_stride; c->token_stride = token_stride;
     c->box_rows = 16;
@@ -229,7 +229,7 @@ extern "C" int ojas_b200_kv_append(ojas_b200_ctx *ctx, const ojas_b200_kv *kv, c
                                    uint32_t q_type, void *q_out, size_t q_out_stride, size_t q_heads, const int32_t *pos, size_t M) {
     if (!ctx) return OJAS_B200_E_ARG;
     if (!kv) return ojas_fail(ctx, OJAS_B200_E_ARG, "kv_append: null cache");
-    if (kv->ctx->device != ctx->device || (rope && rope->ctx->device != ctx->device))
+    if (kv->device != ctx->device || (rope && rope->device != ctx->device))
         return ojas_fail(ctx, OJAS_B200_E_ARG, "kv_append: the cache or the rotation lives on another device than the context's (%d)", ctx->device);
     char why[256];
     const int rc = ojas_b200_kv_append_check(kv->heads, kv->dim, rope ? rope->rot_dim : 0, layout, x_type, q, q_stride, k, k_stride, v, v_stride, q_type, q_out,

@@ -65,7 +65,7 @@ extern "C" int ojas_b200_rope_create(ojas_b200_ctx *ctx, size_t rot_dim, double 
     }
     ojas_b200_rope *r = new (std::nothrow) ojas_b200_rope();
     if (!r) { cudaFree(dev); return ojas_fail(ctx, OJAS_B200_E_LIMIT, "rope_create: out of host memory"); }
-    r->ctx = ctx; r->rot_dim = (uint32_t)rot_dim; r->turns = dev;
+    r->device = ctx->device; r->rot_dim = (uint32_t)rot_dim; r->turns = dev;
     r->magnitude = scaling ? scaling->magnitude : 1.0f;
     *out = r;
     return 0;
@@ -73,7 +73,7 @@ extern "C" int ojas_b200_rope_create(ojas_b200_ctx *ctx, size_t rot_dim, double 
 
 extern "C" void ojas_b200_rope_destroy(ojas_b200_rope *r) {
     if (!r) return;
-    DeviceGuard guard(r->ctx->device);
+    DeviceGuard guard(r->device);
     cudaFree(r->turns);
     delete r;
 }
@@ -123,7 +123,7 @@ extern "C" int ojas_b200_rope_rows(ojas_b200_ctx *ctx, const ojas_b200_rope *rop
                                    uint32_t y_type, void *y, size_t y_stride, const int32_t *pos, size_t M, size_t heads, size_t dim) {
     if (!ctx) return OJAS_B200_E_ARG;
     if (!rope) return ojas_fail(ctx, OJAS_B200_E_ARG, "rope_rows: null rotation");
-    if (rope->ctx->device != ctx->device) return ojas_fail(ctx, OJAS_B200_E_ARG, "rope_rows: the rotation lives on device %d, the context on %d", rope->ctx->device, ctx->device);
+    if (rope->device != ctx->device) return ojas_fail(ctx, OJAS_B200_E_ARG, "rope_rows: the rotation lives on device %d, the context on %d", rope->device, ctx->device);
     char why[256];
     const int rc = ojas_b200_rope_rows_check(rope->rot_dim, layout, x_type, x, x_stride, y_type, y, y_stride, pos, M, heads, dim, why, sizeof why);
     if (rc) return ojas_fail(ctx, rc, "%s", why);

@@ -405,7 +405,7 @@ class Rope:
         self._h = h
 
     def close(self) -> None:
-        if getattr(self, "_h", None) and self.gpu._ctx:
+        if getattr(self, "_h", None):
             self._l.ojas_b200_rope_destroy(self._h)
         self._h = None
 

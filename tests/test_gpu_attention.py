@@ -418,3 +418,106 @@ def test_a_layer_from_its_input_to_the_output_projection(gpu):
 
 def qkv_part(b, floats):
     return ob.Buf(b.ptr + 4 * floats, b.nbytes - 4 * floats)
+
+
+@pytest.mark.parametrize("rows", [1, 80])
+@pytest.mark.parametrize("scale", [0.0, -0.09, 1.0])
+def test_scales(gpu, rows, scale):
+    """Scale 0 gives the mean of the values that are seen; a negative one turns the order round."""
+    b = Batch([rows, 2], [400, 170], kv_heads=2, dim=128, seed=2).upload(gpu)
+    run_attention(gpu, b, 8, F32, scale=scale)
+    run_attention(gpu, b, 8, F16, scale=scale)
+
+
+@pytest.mark.parametrize("rows,dim", [(1, 128), (4, 64), (90, 128), (40, 256)])
+def test_a_row_of_nan_stays_alone(gpu, rows, dim):
+    """A query that is not a number makes its own output so and nothing else."""
+    b = Batch([rows, rows], [300, 200], kv_heads=2, dim=dim, seed=2).upload(gpu)
+    q = randn(torch.Generator().manual_seed(3), b.M, 4, dim)
+    bad = q.clone()
+    bad[rows, 1, 5] = math.nan
+    got = []
+    for t in (q, bad):
+        qd, out = t.cuda(), torch.empty(b.M, 4, dim).cuda()
+        torch.cuda.synchronize()
+        gpu.attention(b.kv, b.seqs, buf(qd), buf(out), b.M, 4)
+        gpu.sync()
+        got.append(out)
+    assert got[1][rows, 1].isnan().all()
+    got[1][rows, 1] = got[0][rows, 1]
+    want, weight, vmax = b.attention_exact(q, 4)             # (a neighbour may move the point a row's exponentials are taken from: not bit for bit)
+    for t in got:
+        check(t, want, attention_bound(want, weight, vmax, dim, 300, F32, F16, 2))
+
+
+@pytest.mark.parametrize("rows,n", [(1, 4), (6, 3), (100, 2)])
+def test_more_rows_than_promised_are_reported(gpu, rows, n):
+    """max_rows below a sequence's new rows, and offsets out of order: an error, and nothing outside the call is touched."""
+    for cu in (None, [0] + [n * rows - i for i in range(n)]):
+        b = Batch([rows] * n, [200] * n, kv_heads=1, dim=64, seed=2, max_rows=max(1, rows // 2), extra_rows=2)
+        if cu:
+            b.cu = torch.tensor(cu, dtype=torch.int32)
+        elif rows == 1:
+            continue
+        b.upload(gpu)
+        q, out = torch.randn(b.M, 4, 64).cuda(), torch.full((b.M + 4, 4, 64), 77.0).cuda()
+        torch.cuda.synchronize()
+        gpu.attention(b.kv, b.seqs, buf(q), buf(out), b.M, 4)
+        p = buf(q)
+        gpu.kv_append(b.kv, b.seqs, p, p, b.M, x_stride=256)
+        with pytest.raises(ob.OjasB200Error):              # (the first sequence has more rows than max_rows either way)
+            gpu.sync()
+        assert (out[b.M :] == 77).all()
+
+
+def test_a_cache_beyond_32_bits(gpu):
+    """Pages more than 2^31 elements and 2^32 bytes from the start."""
+    pages, page, dim = 70000, 256, 128
+    k, v = (torch.empty(pages, page, 1, dim, dtype=torch.float16, device="cuda") for _ in range(2))
+    kv = ob.KvCache(gpu, F16, buf(k), buf(v), pages, page, 1, dim, page_stride=page * dim, head_stride=dim, token_stride=dim)
+    g = torch.Generator().manual_seed(1)
+    table, n = [69999, 3, 69000], 600
+    kr, vr = (randn(g, 3 * page, 1, dim, dtype=torch.float16) for _ in range(2))
+    for i, p in enumerate(table):
+        k[p], v[p] = kr[i * page : (i + 1) * page].cuda(), vr[i * page : (i + 1) * page].cuda()
+    dev = [torch.tensor(t, dtype=torch.int32).cuda() for t in ([0, 30], [n], table)]
+    seqs = ob.Seqs(buf(dev[0]), buf(dev[1]), buf(dev[2]), 1, 3, 30, n)
+    x = randn(g, 30, 6, dim)
+    xd, qo, out = x.cuda(), torch.empty(30, 4, dim).cuda(), torch.empty(30, 4, dim).cuda()
+    p = buf(xd)
+    torch.cuda.synchronize()
+    gpu.kv_append(kv, seqs, ob.Buf(p.ptr + 4 * dim * 4, 0), ob.Buf(p.ptr + 5 * dim * 4, 0), 30, x_stride=6 * dim, q=p, q_out=buf(qo), q_heads=4)
+    gpu.attention(kv, seqs, buf(qo), buf(out), 30, 4)
+    gpu.sync()
+    b = Batch([30], [n], kv_heads=1, dim=dim, page=256)
+    b.k_rows, b.v_rows = [kr[:n].clone()], [vr[:n].clone()]
+    b.k_rows[0][n - 30 :], b.v_rows[0][n - 30 :] = x[:, 4:5].half(), x[:, 5:6].half()
+    assert torch.equal(k[69000, : n - 512].cpu(), b.k_rows[0][512:n])
+    want, weight, vmax = b.attention_exact(x[:, :4], 4)
+    check(out, want, attention_bound(want, weight, vmax, dim, n, F32, F16, 2))
+
+
+@pytest.mark.parametrize("act,cache", TYPES)
+@pytest.mark.parametrize("dim,group,rows,length,kv_heads", [(128, 8, 1, 9000, 1), (64, 4, 40, 6000, 1), (128, 2, 100, 4000, 1), (256, 8, 12, 5000, 1), (128, 5, 3, 20000, 2)])
+def test_split_keys(gpu, act, cache, dim, group, rows, length, kv_heads):
+    """Few tiles over long sequences: every kernel with its keys split, and joined, beside a short sequence that is not."""
+    b = Batch([rows, 1], [length, 3], kv_heads=kv_heads, dim=dim, page=64, cache=cache, seed=length).upload(gpu)
+    run_attention(gpu, b, kv_heads * group, act)
+
+
+def test_two_streams_at_once(gpu):
+    """Two contexts on two streams, each with its own workspace, over the same cache."""
+    b = Batch([1, 1], [9000, 4000], kv_heads=2, dim=128, seed=5).upload(gpu)
+    q = randn(torch.Generator().manual_seed(3), b.M, 8, 128)
+    want, weight, vmax = b.attention_exact(q, 8)
+    qd = q.cuda()
+    others = [ob.B200Gpu(0) for _ in range(2)]
+    outs = [torch.empty(b.M, 8, 128).cuda() for _ in others]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for o, out in zip(others, outs):
+            o.attention(b.kv, b.seqs, buf(qd), buf(out), b.M, 8)
+    for o, out in zip(others, outs):
+        o.sync()
+        check(out, want, attention_bound(want, weight, vmax, 128, 9000, F32, F16, 2))
+        o.close()
