@@ -249,12 +249,13 @@ def extra_gemv(gpu, ob, ggml_type: int, n: int, k: int, m: int, peak: float, tag
             "frac_of_peak": round(gbs / peak, 4), "ring": ring}
 
 
-def decode_layer_case(gpu, ob, peak: float) -> dict:
+def decode_layer_case(gpu, ob, peak: float, context: int = 0) -> dict:
     """The matmul chain of one decode step of an 8B-shaped layer (d = 4096, ffn = 14336, 32 / 8 heads): fused Q|K|V GEMV
     (6144 rows) with the RMSNorm in its prologue, O projection, fused gate|up GEMV (28672 rows) with the RMSNorm in its
     prologue, SiLU * up -> Q8_K, down (Q6_K); also timed with the norms as launches of their own (RMSNorm -> Q8_K) and
     with SiLU * up in the down projection's prologue as well (slower: every CTA repeats the exponentials).  Three layers of distinct weights (414 MB > L2) in one
-    CUDA graph; attention itself is not on this path (the O projection reads the first 4096 QKV outputs instead)."""
+    CUDA graph; the O projection reads the first 4096 QKV outputs.  With a context (`--case layer:CONTEXT`) the whole layer is
+    timed instead: Q and K rotated and K, V appended to a paged f16 cache of that length, attention over it, its result into the O projection."""
     import oracle
     d, ffn, nq = 4096, 14336, 6144
     nsb_d, nsb_f = d // 256, ffn // 256
@@ -273,9 +274,27 @@ def decode_layer_case(gpu, ob, peak: float) -> dict:
     qkv, attn, gu, y = gpu.alloc(nq), gpu.alloc(d), gpu.alloc(2 * ffn), gpu.alloc(d)
     g_view, u_view = ob.Buf(gu.ptr, ffn * 4), ob.Buf(gu.ptr + ffn * 4, ffn * 4)
 
+    if context:
+        page, pages = 64, (context + 63) // 64
+        rope = ob.Rope(gpu, 128, base=500000.0)
+        one = np.arange(pages, dtype=np.int32)
+        seqs = ob.Seqs(gpu.upload(np.array([0, 1], np.int32)), gpu.upload(np.array([context], np.int32)), gpu.upload(rng.permutation(one)), 1, pages, 1, context)
+        caches = []
+        for _ in layers:
+            half = rng.standard_normal(pages * 8 * page * 128, dtype=np.float32).astype(np.float16)
+            caches.append(ob.KvCache(gpu, ob.F16, gpu.upload(half), gpu.upload(half[::-1]), pages, page, 8, 128))
+        turned, mixed = gpu.alloc(d), gpu.alloc(d)
+        k_part, v_part = ob.Buf(qkv.ptr + 4 * 4096, 4 * 2048), ob.Buf(qkv.ptr + 4 * 5120, 4 * 1024)
+
     def chain():
-        for wqkv, wo, wgu, wdn in layers:
-            if fused_norm:
+        for i, (wqkv, wo, wgu, wdn) in enumerate(layers):
+            if context:
+                gpu.gemv_rmsnorm(wqkv, x, nw, 1e-5, qkv)
+                gpu.kv_append(caches[i], seqs, k_part, v_part, 1, rope=rope, x_stride=nq, q=qkv, q_out=turned, q_heads=32)
+                gpu.attention(caches[i], seqs, turned, mixed, 1, 32)
+                gpu.gemv(wo, mixed, attn)
+                gpu.gemv_rmsnorm(wgu, attn, nw, 1e-5, gu)
+            elif fused_norm:
                 gpu.gemv_rmsnorm(wqkv, x, nw, 1e-5, qkv)
                 gpu.gemv(wo, qkv, attn)
                 gpu.gemv_rmsnorm(wgu, attn, nw, 1e-5, gu)
@@ -292,12 +311,14 @@ def decode_layer_case(gpu, ob, peak: float) -> dict:
                 gpu.gemv_q8k(wdn, q_f, s_f, b_f, y)
 
     us = {}
-    for fused_norm in (0, 1, 2):        # producers as launches of their own; norms in the GEMV prologues; SwiGLU too
+    for fused_norm in (1,) if context else (0, 1, 2):        # producers as launches of their own; norms in the GEMV prologues; SwiGLU too
         chain()
         gpu.sync()
+        before = gpu.launch_count
         gpu.graph_begin()
         chain()
         g = gpu.graph_end()
+        launches = (gpu.launch_count - before) // len(layers)
         ms = time_graph(gpu, g, 300, 5)
         gpu.graph_destroy(g)
         us[fused_norm] = ms * 1e3 / 300 / len(layers)
@@ -308,6 +329,13 @@ def decode_layer_case(gpu, ob, peak: float) -> dict:
             gpu.free(w.buf)
     for b in (x, nw, q_d, s_d, b_d, q_f, s_f, b_f, qkv, attn, gu, y):
         gpu.free(b)
+    if context:
+        kv_bytes = 2 * 2 * 8 * 128 * context
+        for b in (seqs.cu, seqs.lens, seqs.table, turned, mixed, *(h for c in caches for h in (c.k, c.v))):
+            gpu.free(b)
+        return {"workload": f"decode_layer_d4096_ffn14336_q4k_q6k_m1_context{context}", "us_per_layer": round(us_layer, 2), "launches_per_layer": launches,
+                "GB/s": round((gguf + kv_bytes) / us_layer / 1e3, 1), "frac_of_peak": round((gguf + kv_bytes) / us_layer / 1e3 / peak, 4),
+                "weight_bytes": gguf, "kv_bytes": kv_bytes}
     return {"workload": "decode_layer_d4096_ffn14336_q4k_q6k_m1", "us_per_layer": round(us_layer, 2), "launches_per_layer": 5,
             "us_per_layer_with_separate_producer_launches": round(us[0], 2), "us_per_layer_with_swiglu_fused_too": round(us[2], 2),
             "GB/s": round(gguf / us_layer / 1e3, 1), "frac_of_peak": round(gguf / us_layer / 1e3 / peak, 4), "weight_bytes": gguf}
@@ -533,10 +561,10 @@ def run_case(args) -> None:
         return run_gemm_case(args)
     if args.case == "tp70b":
         return run_tp70b(args)
-    if args.case == "layer":
+    if args.case == "layer" or args.case.startswith("layer:"):
         hbm_peak, _, _ = measured_peaks()
         gpu = ob.B200Gpu(0)
-        print(json.dumps(decode_layer_case(gpu, ob, hbm_peak)))
+        print(json.dumps(decode_layer_case(gpu, ob, hbm_peak, int(args.case.split(":")[1]) if ":" in args.case else 0)))
         gpu.close()
         return
     if args.case == "moe" or args.case.startswith("moe:"):

@@ -476,7 +476,8 @@ static AttnPlan attn_plan(int sm_count, size_t n_seqs, size_t M, size_t max_rows
     p.rows = p.tensor ? (dim == 256 || f32 ? 128 : 256) : (int)unit * p.mt;
     p.block = p.tensor && dim != 256 ? 128 : 64;
     const unsigned long long by_seq = (unsigned long long)n_seqs * ((bound + p.rows - 1) / p.rows), by_row = (unsigned long long)M * group / p.rows + n_seqs;
-    p.tiles = (long long)(by_seq < by_row ? by_seq : by_row);
+    p.tiles = (long long)(by_seq <= by_row ? by_seq : by_row);
+    p.per_seq = by_seq <= by_row ? (int)((bound + p.rows - 1) / p.rows) : 0;
     size_t span = max_len;                                   // keys a tile can see at most
     if (window && window + p.rows < span) span = window + p.rows;
     const double blocks = (double)(span / p.block + 2), ctas = (double)p.tiles * (double)kv_heads;
@@ -581,14 +582,14 @@ extern "C" int ojas_b200_attention(ojas_b200_ctx *ctx, const ojas_b200_kv *kv, c
         if (!workspace || workspace_bytes < p.workspace) return ojas_fail(ctx, OJAS_B200_E_ARG, "attention: workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : 0, p.workspace);
         if ((uintptr_t)workspace % 256) return ojas_fail(ctx, OJAS_B200_E_ARG, "attention: the workspace must start on 256 bytes");
     }
-    if (p.tiles > 0x7fffffffll || p.splits > 65535) return ojas_fail(ctx, OJAS_B200_E_LIMIT, "attention: too many row tiles");
+    if (p.tiles * (long long)kv->heads > 0x7fffffffll || p.splits > 65535) return ojas_fail(ctx, OJAS_B200_E_LIMIT, "attention: too many row tiles");
     AttnArgs a{};
     a.q = q; a.out = out;
     a.q_stride = (long long)(q_stride ? q_stride : q_heads * kv->dim);
     a.out_stride = (long long)(out_stride ? out_stride : q_heads * kv->dim);
     a.batch = {seqs->cu, seqs->len, seqs->table, (int)seqs->n_seqs, (int)seqs->table_stride, (long long)M, (int)kv->pages, (int)kv->page_size, (int)seqs->max_rows, ctx->dev_status};
     a.act_type = act_type; a.q_heads = (int)q_heads; a.group = (int)(q_heads / kv->heads);
-    a.splits = p.splits; a.split_blocks = p.split_blocks;
+    a.splits = p.splits; a.split_blocks = p.split_blocks; a.per_seq = p.per_seq;
     a.window = (int)window; a.causal = causal != 0;
     a.scale_log2 = scale * 1.4426950408889634f;
     if (p.workspace) {

@@ -15,13 +15,14 @@ struct AttnArgs {
     uint32_t act_type;
     int q_heads, group;                  // group = query heads per key head
     int splits, split_blocks;            // key blocks per split
+    int per_seq;                         // row tiles of every sequence (0: as many as its rows need)
     int window;                          // 0: none
     bool causal;
     float scale_log2;                    // softmax scale * log2(e)
 };
 
 // A row is one (token, query head) pair; the rows of a sequence that share a key head are numbered token * group + head in
-// group, and a tile is `rows` of them.  Tile t of the call belongs to the sequence found by walking the row counts.
+// group, and a tile is `rows` of them.
 struct RowTile {
     int seq, row0, n_rows;               // first row in the sequence, rows of the sequence (all of them)
     int token0;                          // call row of the sequence's first new token
@@ -29,44 +30,70 @@ struct RowTile {
     int len;                             // keys that may be read
 };
 
-// One warp, all lanes: which sequence tile `tile` (counted over all sequences) falls in.  False: behind the last one.
-// Every value is clamped so that no description, however wrong, leads outside the arrays; a wrong one sets the status bit.
+// First row and number of rows of sequence s, clamped to the call.
+__device__ __forceinline__ void seq_rows(const BatchArgs &b, int s, int &first, int &n) {
+    first = max(0, __ldg(b.cu + s));
+    n = (int)max(0ll, min((long long)__ldg(b.cu + s + 1), b.M) - first);
+}
+
+// One warp, all lanes: which rows tile `tile` of the call is.  With per_seq > 0 every sequence has that many tiles, used or not; else
+// tiles are counted over the sequences' rows, 128 sequences at a time.  False: no such rows.  Every value is clamped so that no
+// description, however wrong, leads outside the arrays; a wrong one sets the status bit.
 __device__ __forceinline__ bool find_tile(const AttnArgs &a, int tile, int rows, int lane, RowTile &t) {
     const BatchArgs &b = a.batch;
-    long long before = 0;
-    for (int s0 = 0; s0 < b.n_seqs; s0 += 32) {
-        const int s = s0 + lane;
-        long long first = 0, n = 0;
-        if (s < b.n_seqs) {
-            first = max(0, __ldg(b.cu + s));
-            n = min((long long)__ldg(b.cu + s + 1), b.M) - first;
-            n = n < 0 ? 0 : n;
-        }
-        const int tiles = (int)((n * a.group + rows - 1) / rows);
-        int sum = tiles;                                          // inclusive prefix over the lanes
+    int first = 0, n = 0;
+    long long before = 0;                                         // tiles of the sequences in front
+    if (a.per_seq > 0) {
+        t.seq = tile / a.per_seq;
+        if (t.seq >= b.n_seqs) return false;
+        before = (long long)t.seq * a.per_seq;
+        seq_rows(b, t.seq, first, n);
+    } else {
+        bool found = false;
+        for (int s0 = 0; s0 < b.n_seqs && !found; s0 += 128) {
+            int start[4], count[4], tiles[4], sum = 0;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, sum, o);
-            if (lane >= o) sum += v;
+            for (int i = 0; i < 4; i++) {
+                const int s = s0 + lane * 4 + i;
+                start[i] = count[i] = 0;
+                if (s < b.n_seqs) seq_rows(b, s, start[i], count[i]);
+                tiles[i] = (int)(((long long)count[i] * a.group + rows - 1) / rows);
+                sum += tiles[i];
+            }
+            int upto = sum;                                       // inclusive prefix over the lanes
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += v;
+            }
+            const unsigned hit = __ballot_sync(0xffffffffu, before + upto > tile);
+            if (hit) {
+                const int src = __ffs(hit) - 1;
+                long long at = before + upto - sum;               // the lane's own sequences
+                int which = 0;
+#pragma unroll
+                for (int i = 0; i < 3; i++)
+                    if (which == i && at + tiles[i] <= tile) { at += tiles[i]; which = i + 1; }
+                t.seq = s0 + src * 4 + __shfl_sync(0xffffffffu, which, src);
+                first = __shfl_sync(0xffffffffu, which == 0 ? start[0] : which == 1 ? start[1] : which == 2 ? start[2] : start[3], src);
+                n = __shfl_sync(0xffffffffu, which == 0 ? count[0] : which == 1 ? count[1] : which == 2 ? count[2] : count[3], src);
+                before = __shfl_sync(0xffffffffu, at, src);
+                found = true;
+            } else {
+                before += __shfl_sync(0xffffffffu, upto, 31);
+            }
         }
-        const unsigned hit = __ballot_sync(0xffffffffu, before + sum > tile);
-        if (hit) {
-            const int src = __ffs(hit) - 1;
-            t.seq = s0 + src;
-            t.token0 = (int)__shfl_sync(0xffffffffu, first, src);
-            const int tokens = (int)__shfl_sync(0xffffffffu, n, src);
-            t.n_rows = tokens * a.group;
-            t.row0 = (int)(tile - before - __shfl_sync(0xffffffffu, sum - tiles, src)) * rows;
-            const int len = __ldg(b.len + t.seq);
-            const long long room = (long long)b.table_stride * b.page_size;
-            t.pos0 = len - tokens;
-            t.len = (int)max(0ll, min((long long)len, room));
-            if (lane == 0 && ((long long)len > room || len < tokens || tokens > b.max_rows)) atomicOr(b.status, OJAS_ST_BATCH);
-            return t.row0 >= 0 && t.row0 < t.n_rows;              // (offsets out of order could overflow the count)
-        }
-        before += __shfl_sync(0xffffffffu, sum, 31);
+        if (!found) return false;
     }
-    return false;
+    t.token0 = first;
+    t.n_rows = n * a.group;
+    t.row0 = (int)(tile - before) * rows;
+    const int len = __ldg(b.len + t.seq);
+    const long long room = (long long)b.table_stride * b.page_size;
+    t.pos0 = len - n;
+    t.len = (int)max(0ll, min((long long)len, room));
+    if (lane == 0 && n > 0 && ((long long)len > room || len < n || n > b.max_rows)) atomicOr(b.status, OJAS_ST_BATCH);
+    return t.row0 >= 0 && t.row0 < t.n_rows;                      // (offsets out of order could overflow the count)
 }
 
 // Keys [lo, hi) that rows [row0, row1) of the tile's sequence see, taken together (empty: hi <= lo).
@@ -100,6 +127,7 @@ struct AttnPlan {
     bool two, cluster;                   // the kernel for few rows: two terms per value; the splits are a cluster
     int rows, mt;                        // rows of a tile; MMA tiles per warp of the kernel for few rows
     long long tiles;                     // upper bound on the call's row tiles
+    int per_seq;                         // see AttnArgs
     int splits, split_blocks, block;     // keys per block
     size_t workspace;
 };
