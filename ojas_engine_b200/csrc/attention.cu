@@ -16,17 +16,17 @@
 // activations use all 16 rows and round the probabilities once.  f32 rows are scaled by a power of two first so that neither term
 // leaves f16's range; probabilities are kept scaled by 2^8 for the same reason.
 //
-// Keys are split over CTAs where there are few tiles.  Up to eight splits that all fit on the GPU at once form a cluster and join
-// through each other's shared memory (one short sequence: 9.9 -> 8.3 us); otherwise they write their sums to the workspace and a second
+// Keys are split over CTAs where there are few tiles.  Up to 16 splits that all fit on the GPU at once form a cluster and join
+// through each other's shared memory (one short sequence: 9.9 -> 7.2 us); otherwise they write their sums to the workspace and a second
 // kernel joins them (CTAs of a cluster hold their places until the last of them is there: 64 ragged sequences in four
-// splits take 272 us as clusters, 193 us this way).
+// splits take 272 us as clusters, 186 us this way).
 #include "attention.cuh"
 
 // ---------------------------------------------------------------------------- few rows: warp-level MMA
 constexpr int AR_KEYS = 64;                                  // keys of a block
 constexpr int AR_WARPS = 4, AR_THREADS = (AR_WARPS + 1) * 32;   // consumer warps; and the producer
 constexpr int AR_STAT_BYTES = 256 + AR_WARPS * 32 * 8 + 32 * 8;   // barriers; per warp and row (maximum, sum); per row the same
-constexpr int AR_CLUSTER = 8;                                // splits that can be a cluster
+constexpr int AR_CLUSTER = 16;                               // splits that can be a cluster (above 8: allowed on this architecture when asked for)
 __host__ __device__ constexpr int ar_stage_bytes(int dim) { return 2 * AR_KEYS * dim * 2; }
 // 96 KB of blocks in flight per CTA, two CTAs per SM (dim 256: three 64 KB blocks, one CTA): HBM needs about 44 KB per SM and
 // microsecond of latency.
@@ -483,8 +483,8 @@ static AttnPlan attn_plan(int sm_count, size_t n_seqs, size_t M, size_t max_rows
     const double blocks = (double)(span / p.block + 2), ctas = (double)p.tiles * (double)kv_heads;
     // Times in key blocks (about 1.5 us).  A CTA costs its start and end, hidden by its neighbour where two share an SM, and its blocks.
     // Lengths are bounds: of many sequences most are shorter, about half as long on average.  CTAs are handed to `slots` places as
-    // they come free, so that the last ends about half a CTA after the work would on average.  Splits cost a launch, and the bytes of
-    // their sums.  (One 131 000-key pair of sequences: 135 us in 16 to 18 splits, 150 in 63; 64 ragged sequences of up to 8192
+    // they come free, so that the last ends about half a CTA after the work would on average.  Splits that do not join as a cluster
+    // cost a launch, and the bytes of their sums.  (One 131 000-key pair of sequences: 135 us in 16 to 18 splits, 150 in 63; 64 ragged sequences of up to 8192
     // keys: 202 us in one split, 186 in 3 or 4, 214 in 12; 16 of up to 6000 with dim 256: 132, 43 in 4, 37 in 6, 50 in 16.)
     const bool pairs = dim != 256 && p.mt == 1 && !p.tensor;
     const double slots = (double)sm_count * (pairs ? 2 : 1), fixed = pairs ? 3.0 : 6.0, part = 0.5 + 0.5 / (double)n_seqs;
@@ -493,7 +493,8 @@ static AttnPlan attn_plan(int sm_count, size_t n_seqs, size_t M, size_t max_rows
     int splits = 1;
     for (int n = 1; n <= 64 && n * 2 <= (int)blocks; n = n < 8 ? n + 1 : n + n / 4) {
         const double each = fixed + blocks / n, all = ctas * n, spread = part * all * each / slots + 0.5 * each;
-        const double cost = (all <= slots || each > spread ? each : spread) + (n > 1 ? 3.0 + sums * n : 0.0);
+        const bool cluster = !p.tensor && n <= AR_CLUSTER && all <= slots;
+        const double cost = (all <= slots || each > spread ? each : spread) + (n == 1 ? 0.0 : cluster ? 0.1 * n : 3.0 + sums * n);
         if (n == 1 || cost < best) { best = cost; splits = n; }
     }
     p.split_blocks = (int)((blocks + splits - 1) / splits);
@@ -535,7 +536,7 @@ extern "C" size_t ojas_b200_attention_workspace_bytes(ojas_b200_ctx *ctx, const 
 template <int D, bool BF, bool TWO, int MT>
 static cudaError_t launch_rows(const ojas_b200_ctx *ctx, const ojas_b200_kv *kv, const AttnArgs &a, const AttnPlan &p) {
     static std::atomic<uint64_t> ready{0};
-    const cudaError_t e = smem_once(ready, ctx->device, attn_rows_kernel<D, BF, TWO, MT>, ar_smem(D));
+    const cudaError_t e = smem_once(ready, ctx->device, attn_rows_kernel<D, BF, TWO, MT>, ar_smem(D), p.cluster && p.splits > 8);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)p.tiles, (unsigned)kv->heads, (unsigned)p.splits);

@@ -111,13 +111,15 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
-// Allows a kernel its dynamic shared memory, once per device (a bit each; devices from 64 on are asked every time).
+// Allows a kernel its dynamic shared memory, and clusters of more than eight CTAs, once per device (two bits each; devices from
+// 32 on are asked every time).
 template <typename K>
-static cudaError_t smem_once(std::atomic<uint64_t> &ready, int device, K kernel, int bytes) {
-    const uint64_t bit = device < 64 ? 1ull << device : 0ull;
-    if (bit && (ready.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e == cudaSuccess) ready.fetch_or(bit, std::memory_order_relaxed);
+static cudaError_t smem_once(std::atomic<uint64_t> &ready, int device, K kernel, int bytes, bool large_clusters = false) {
+    const uint64_t bit = device < 32 ? 1ull << (2 * device) : 0ull, want = large_clusters ? 3 * bit : bit;
+    if (bit && (ready.load(std::memory_order_relaxed) & want) == want) return cudaSuccess;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && large_clusters) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess) ready.fetch_or(want, std::memory_order_relaxed);
     return e;
 }
 

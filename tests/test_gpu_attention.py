@@ -297,7 +297,7 @@ def test_bounds_larger_than_the_batch(gpu):
 
 
 def test_workspace_is_checked(gpu):
-    b = Batch([1], [4000], kv_heads=2, dim=128, seed=2).upload(gpu)
+    b = Batch([1], [4000], kv_heads=2, dim=128, seed=2, max_len=400000).upload(gpu)     # a bound that asks for more splits than join in one launch
     need = gpu.attention_workspace_bytes(b.kv, b.seqs, 1, 8)
     assert need > 0
     q, out, ws = torch.zeros(8, 128).cuda(), torch.zeros(8, 128).cuda(), torch.zeros(need + 256, dtype=torch.uint8).cuda()
