@@ -129,67 +129,70 @@ struct AppendArgs {
     long long q_stride, k_stride, v_stride, q_out_stride, page_stride, head_stride, token_stride;
     BatchArgs batch;
     uint32_t x_type, q_type, c_type;
-    int q_heads, kv_heads, dim, rot, tokens_per_cta;
+    int q_heads, kv_heads, dim, rot;
     bool interleaved;
 };
-constexpr int APPEND_TOKENS = 8;       // most tokens of a CTA: one warp looks up each
 
+// One CTA per token, as rope_rows: the first loads of q, k and v go out before the token's place is looked up.
 template <int VEC>
 __global__ void __launch_bounds__(256) kv_append_kernel(const AppendArgs a) {
-    extern __shared__ float2 append_cs[];                // [tokens_per_cta][rot / 2]
-    __shared__ long long row_at[APPEND_TOKENS];          // element offset of the token's row of head 0 in the cache; -1: not written
-    __shared__ int row_pos[APPEND_TOKENS];               // position of rotation
-    __shared__ bool row_live[APPEND_TOKENS];             // the row belongs to a sequence
+    extern __shared__ float2 append_cs[];                // [rot / 2]
+    __shared__ long long row_at_s;                       // element offset of the token's row of head 0 in the cache; -1: not written
+    __shared__ int row_pos_s;                            // position of rotation
+    __shared__ bool row_live_s;                          // the row belongs to a sequence
     grid_launch_dependents();
     grid_dependency_wait();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const long long t0 = (long long)blockIdx.x * a.tokens_per_cta;
-    const int tokens = (int)min((long long)a.tokens_per_cta, a.batch.M - t0);
-    if (warp < tokens) {
-        const long long t = t0 + warp;
+    const int lane = threadIdx.x & 31;
+    const long long t = blockIdx.x;
+    const int rot = a.turns ? a.rot : 0, units = rope_units(VEC, rot, a.dim);
+    const int ux = threadIdx.x % units, uy = threadIdx.x / units, ny = blockDim.x / units;   // (dim <= 256: at most 128 units)
+    const RopeUnit<VEC> unit(uy < ny ? ux : units, rot, a.dim, a.interleaved), plain(uy < ny ? ux : units, 0, a.dim, false);   // (a thread too many has nothing)
+    typename RopeUnit<VEC>::Parts p[ROPE_BATCH], k, v;
+    const long long qo = t * a.q_stride, ko = t * a.k_stride, vo = t * a.v_stride;
+    rope_fetch(unit, uy, ny, a.q_heads, a.dim, a.q, a.x_type, qo, p);
+    if (uy < a.kv_heads) {
+        unit.fetch(a.k, a.x_type, ko + uy * a.dim, k);
+        plain.fetch(a.v, a.x_type, vo + uy * a.dim, v);
+    }
+    if (threadIdx.x < 32) {
         const int b = find_seq(a.batch.cu, a.batch.n_seqs, t, lane);
         if (lane == 0) {
             long long at = -1;
             int pos = 0;
             if (b >= 0) {
                 const int first = __ldg(a.batch.cu + b), end = __ldg(a.batch.cu + b + 1);
-                const long long p = (long long)__ldg(a.batch.len + b) - end + t;       // = len - rows + (t - first)
-                const long long entry = p / a.batch.page_size;
+                const long long at_pos = (long long)__ldg(a.batch.len + b) - end + t;      // = len - rows + (t - first)
+                const long long entry = at_pos / a.batch.page_size;
                 int page = -1;
-                if (p >= 0 && first >= 0 && entry < a.batch.table_stride) page = __ldg(a.batch.table + (long long)b * a.batch.table_stride + entry);
-                if (page >= 0 && page < a.batch.pages) at = (long long)page * a.page_stride + (p - entry * a.batch.page_size) * a.token_stride;
-                else atomicOr(a.batch.status, OJAS_ST_BATCH);                          // nowhere to put it: q is still turned
-                pos = a.pos ? __ldg(a.pos + t) : (int)p;
+                if (at_pos >= 0 && first >= 0 && entry < a.batch.table_stride) page = __ldg(a.batch.table + (long long)b * a.batch.table_stride + entry);
+                if (page >= 0 && page < a.batch.pages) at = (long long)page * a.page_stride + (at_pos - entry * a.batch.page_size) * a.token_stride;
+                else atomicOr(a.batch.status, OJAS_ST_BATCH);                              // nowhere to put it: q is still turned
+                pos = a.pos ? __ldg(a.pos + t) : (int)at_pos;
             }
-            row_live[warp] = b >= 0;
-            row_at[warp] = at;
-            row_pos[warp] = pos;
+            row_live_s = b >= 0;
+            row_at_s = at;
+            row_pos_s = pos;
         }
     }
     __syncthreads();
-    const int half = a.turns ? a.rot >> 1 : 0;
-    for (int i = threadIdx.x; i < tokens * half; i += blockDim.x) {
-        const int t = i / half, f = i - t * half;
-        append_cs[i] = rope_angle(row_pos[t], __ldg(a.turns + f), a.magnitude);
-    }
+    if (!row_live_s) return;
+    for (int f = threadIdx.x; f < rot >> 1; f += blockDim.x) append_cs[f] = rope_angle(row_pos_s, __ldg(a.turns + f), a.magnitude);
     __syncthreads();
-    const int rot = a.turns ? a.rot : 0, turning = rope_units(VEC, rot, a.dim);
-    const int ux = threadIdx.x % turning, uy = threadIdx.x / turning, ny = blockDim.x / turning;   // (dim <= 256: at most 128 units)
-    if (uy >= ny) return;
-    const RopeUnit<VEC> unit(ux, rot, a.dim, a.interleaved), plain(ux, 0, a.dim, false);
-    for (int t = 0; t < tokens; t++) {
-        if (!row_live[t]) continue;
-        const long long tok = t0 + t;
-        const float2 *cs = append_cs + t * half;
-#pragma unroll 4
-        for (int h = uy; h < a.q_heads; h += ny)
-            unit.apply(a.q, a.x_type, tok * a.q_stride + h * a.dim, a.q_out, a.q_type, tok * a.q_out_stride + h * a.dim, cs);
-        if (row_at[t] < 0) continue;
+    const long long row_at = row_at_s, q_to = t * a.q_out_stride;
+    if (row_at >= 0) {
         for (int h = uy; h < a.kv_heads; h += ny) {
-            const long long to = row_at[t] + (long long)h * a.head_stride;
-            unit.apply(a.k, a.x_type, tok * a.k_stride + h * a.dim, a.kc, a.c_type, to, cs);
-            plain.apply(a.v, a.x_type, tok * a.v_stride + h * a.dim, a.vc, a.c_type, to, cs);
+            if (h != uy) {
+                unit.fetch(a.k, a.x_type, ko + h * a.dim, k);
+                plain.fetch(a.v, a.x_type, vo + h * a.dim, v);
+            }
+            unit.put(k, a.kc, a.c_type, row_at + (long long)h * a.head_stride, append_cs);
+            plain.put(v, a.vc, a.c_type, row_at + (long long)h * a.head_stride, append_cs);
         }
+    }
+    rope_put(unit, uy, ny, a.q_heads, a.dim, a.q_out, a.q_type, q_to, append_cs, p);
+    for (int h = uy + ROPE_BATCH * ny; h < a.q_heads; h += ROPE_BATCH * ny) {
+        rope_fetch(unit, h, ny, a.q_heads, a.dim, a.q, a.x_type, qo, p);
+        rope_put(unit, h, ny, a.q_heads, a.dim, a.q_out, a.q_type, q_to, append_cs, p);
     }
 }
 
@@ -250,12 +253,10 @@ extern "C" int ojas_b200_kv_append(ojas_b200_ctx *ctx, const ojas_b200_kv *kv, c
     a.q_heads = (int)q_heads; a.kv_heads = (int)kv->heads; a.dim = (int)kv->dim;
     const bool vec = rope_vec_ok(a.rot, a.dim, a.interleaved) && rope_rows_aligned(k, x_type, a.k_stride) && rope_rows_aligned(v, x_type, a.v_stride) &&
                      (q_heads == 0 || (rope_rows_aligned(q, x_type, a.q_stride) && rope_rows_aligned(q_out, q_type, a.q_out_stride)));
-    int tpc = M >= (size_t)ctx->sm_count * 16 ? 4 : 1;       // as rope_rows: few tokens spread out, many share a CTA
-    a.tokens_per_cta = tpc;
-    const size_t smem = (size_t)tpc * (a.rot / 2) * sizeof(float2);
+    const size_t smem = (size_t)(a.rot / 2) * sizeof(float2);
     DeviceGuard guard(ctx->device);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((M + tpc - 1) / tpc)); cfg.blockDim = dim3(256); cfg.dynamicSmemBytes = smem; cfg.stream = ctx->stream;
+    cfg.gridDim = dim3((unsigned)M); cfg.blockDim = dim3(256); cfg.dynamicSmemBytes = smem; cfg.stream = ctx->stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;

@@ -88,33 +88,31 @@ struct RopeArgs {
     long long x_stride, y_stride;      // elements between tokens
     long long M;
     uint32_t x_type, y_type;
-    int heads, dim, rot, tokens_per_cta;
+    int heads, dim, rot;
     bool interleaved;
 };
 
-// One CTA takes tokens_per_cta tokens: it forms their cosines and sines once in shared memory, then every thread owns one
-// unit of a head (VEC pairs, or 2 VEC elements that pass through) and walks the (token, head) rows.
+// One CTA per token: its first loads go out, then it forms the token's cosines and sines in shared memory; every thread owns one
+// unit of a head (VEC pairs, or 2 VEC elements that pass through) and walks the heads.  HBM bound: x in, y out.
 template <int VEC>
 __global__ void __launch_bounds__(256) rope_rows_kernel(const RopeArgs a) {
-    extern __shared__ float2 rope_cs[];           // [tokens_per_cta][rot / 2]
+    extern __shared__ float2 rope_cs[];           // [rot / 2]
     grid_launch_dependents();
     grid_dependency_wait();                       // x and pos come from the kernels before this one
-    const int half = a.rot >> 1;
-    const long long t0 = (long long)blockIdx.x * a.tokens_per_cta;
-    const int tokens = (int)min((long long)a.tokens_per_cta, a.M - t0);
-    const int tid = threadIdx.y * blockDim.x + threadIdx.x, threads = blockDim.x * blockDim.y;
-    for (int i = tid; i < tokens * half; i += threads) {
-        const int t = i / half, f = i - t * half;
-        rope_cs[i] = rope_angle(__ldg(a.pos + t0 + t), __ldg(a.turns + f), a.magnitude);
-    }
+    const long long t = blockIdx.x, xo = t * a.x_stride, yo = t * a.y_stride;
+    const int units = rope_units(VEC, a.rot, a.dim), ty = threadIdx.y, ny = blockDim.y;
+    const RopeUnit<VEC> unit(threadIdx.x, a.rot, a.dim, a.interleaved);
+    typename RopeUnit<VEC>::Parts p[ROPE_BATCH];
+    const int pos = __ldg(a.pos + t);
+    rope_fetch(unit, ty, ny, a.heads, a.dim, a.x, a.x_type, xo, p);
+    for (int f = ty * blockDim.x + threadIdx.x; f < a.rot >> 1; f += ny * blockDim.x) rope_cs[f] = rope_angle(pos, __ldg(a.turns + f), a.magnitude);
     __syncthreads();
-    const int units = rope_units(VEC, a.rot, a.dim);
+    rope_put(unit, ty, ny, a.heads, a.dim, a.y, a.y_type, yo, rope_cs, p);
     for (int u = threadIdx.x; u < units; u += blockDim.x) {
-        const RopeUnit<VEC> unit(u, a.rot, a.dim, a.interleaved);
-        for (int t = 0; t < tokens; t++) {
-            const long long xo = (t0 + t) * a.x_stride, yo = (t0 + t) * a.y_stride;
-#pragma unroll 4
-            for (int h = threadIdx.y; h < a.heads; h += blockDim.y) unit.apply(a.x, a.x_type, xo + h * a.dim, a.y, a.y_type, yo + h * a.dim, rope_cs + t * half);
+        const RopeUnit<VEC> part(u, a.rot, a.dim, a.interleaved);
+        for (int h = ty + (u < (int)blockDim.x ? ROPE_BATCH * ny : 0); h < a.heads; h += ROPE_BATCH * ny) {
+            rope_fetch(part, h, ny, a.heads, a.dim, a.x, a.x_type, xo, p);
+            rope_put(part, h, ny, a.heads, a.dim, a.y, a.y_type, yo, rope_cs, p);
         }
     }
 }
@@ -137,16 +135,10 @@ extern "C" int ojas_b200_rope_rows(ojas_b200_ctx *ctx, const ojas_b200_rope *rop
     const bool vec = rope_vec_ok(a.rot, a.dim, a.interleaved) && rope_rows_aligned(x, x_type, a.x_stride) && rope_rows_aligned(y, y_type, a.y_stride);
     const int units = rope_units(vec ? 4 : 1, a.rot, a.dim);
     const dim3 block(units < 256 ? units : 256, units < 256 ? 256 / units : 1);
-    // Few tokens: one per CTA, so that all of them run at once; many: several, so that the sines are formed with every lane
-    // busy.  A CTA's angles have to fit in 16 KB.
-    int tpc = M >= (size_t)ctx->sm_count * 16 ? 4 : 1;
-    while (tpc > 1 && tpc * (a.rot / 2) * (int)sizeof(float2) > 16384) tpc >>= 1;
-    a.tokens_per_cta = tpc;
-    const size_t ctas = (M + tpc - 1) / tpc;
-    const size_t smem = (size_t)tpc * (a.rot / 2) * sizeof(float2);
+    const size_t smem = (size_t)(a.rot / 2) * sizeof(float2);
     DeviceGuard guard(ctx->device);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)ctas); cfg.blockDim = block; cfg.dynamicSmemBytes = smem; cfg.stream = ctx->stream;
+    cfg.gridDim = dim3((unsigned)M); cfg.blockDim = block; cfg.dynamicSmemBytes = smem; cfg.stream = ctx->stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;

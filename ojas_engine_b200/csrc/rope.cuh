@@ -24,32 +24,54 @@ static inline bool rope_rows_aligned(const void *p, uint32_t type, long long str
 
 template <int VEC>
 struct RopeUnit {
-    int a, b, f;         // element offsets of the unit's two parts, index of its first frequency (-1: passes through, -2: nothing)
+    // Element offsets of the unit's two parts, each VEC neighbouring elements so that a warp's accesses are whole stretches of a row;
+    // the first frequencies of the pairs they belong to (f -1: passes through, -2: nothing).
+    int a, b, f, f2;
     bool inter;
     __device__ RopeUnit(int u, int rot, int dim, bool interleaved) : inter(interleaved) {
         const int turning = rot / 2 / VEC;
         if (u < turning) {
-            f = u * VEC;
-            a = interleaved ? 2 * u * VEC : u * VEC;
-            b = interleaved ? a + VEC : a + rot / 2;
+            f = f2 = u * VEC;                                  // half: part a holds the pairs' first members, part b the second
+            a = u * VEC;
+            b = a + rot / 2;
+            if (interleaved && VEC == 4) {                      // two pairs in each part
+                f = 2 * u;
+                f2 = f + rot / 4;
+            } else if (interleaved) {
+                a = 2 * u;
+                b = a + 1;
+            }
         } else {
-            a = rot + (u - turning) * 2 * VEC;
-            b = a + VEC;
-            f = a < dim ? -1 : -2;
+            const int pass = u - turning, step = VEC == 4 ? (dim - rot) / 2 : 1;
+            a = rot + pass * (VEC == 4 ? 4 : 2);
+            b = a + step;
+            f = f2 = b < dim ? -1 : -2;
         }
     }
-    // One head: x at element xo -> y at element yo.  x and y may be the same row: a thread reads all it writes first.
-    __device__ __forceinline__ void apply(const void *x, uint32_t xt, long long xo, void *y, uint32_t yt, long long yo, const float2 *cs) const {
+    // One head's unit: x at element xo -> y at element yo, read and written apart so that a thread can read several heads before it
+    // writes the first (the compiler has to assume that y is x).
+    struct Parts { float4 a, b; };
+    __device__ __forceinline__ void fetch(const void *x, uint32_t xt, long long xo, Parts &p) const {
         if (f == -2) return;
         if (VEC == 4) {
-            const float4 p = load_elem4(x, xt, xo + a), q = load_elem4(x, xt, xo + b);
+            p.a = load_elem4(x, xt, xo + a);
+            p.b = load_elem4(x, xt, xo + b);
+        } else {
+            p.a.x = load_elem(x, xt, xo + a);
+            p.b.x = load_elem(x, xt, xo + b);
+        }
+    }
+    __device__ __forceinline__ void put(const Parts &in, void *y, uint32_t yt, long long yo, const float2 *cs) const {
+        if (f == -2) return;
+        const float4 p = in.a, q = in.b;
+        if (VEC == 4) {
             if (f < 0) {
                 store_elem4(y, yt, yo + a, p);
                 store_elem4(y, yt, yo + b, q);
                 return;
             }
-            const float4 *c4 = reinterpret_cast<const float4 *>(cs + f);
-            const float4 c01 = c4[0], c23 = c4[1];             // (cos, sin) of two frequencies each
+            // (cos, sin) of two frequencies each: pairs 0, 1 and 2, 3 of the unit
+            const float4 c01 = *reinterpret_cast<const float4 *>(cs + f), c23 = *reinterpret_cast<const float4 *>(cs + (inter ? f2 : f + 2));
             float4 u, v;
             if (inter) {                                        // p = pairs 0, 1; q = pairs 2, 3
                 u = make_float4(p.x * c01.x - p.y * c01.y, p.y * c01.x + p.x * c01.y, p.z * c01.z - p.w * c01.w, p.w * c01.z + p.z * c01.w);
@@ -61,15 +83,39 @@ struct RopeUnit {
             store_elem4(y, yt, yo + a, u);
             store_elem4(y, yt, yo + b, v);
         } else {
-            const float p = load_elem(x, xt, xo + a), q = load_elem(x, xt, xo + b);
-            float u = p, v = q;
+            float u = p.x, v = q.x;
             if (f >= 0) {
                 const float2 c = cs[f];
-                u = p * c.x - q * c.y;
-                v = q * c.x + p * c.y;
+                u = p.x * c.x - q.x * c.y;
+                v = q.x * c.x + p.x * c.y;
             }
             store_elem(y, yt, yo + a, u);
             store_elem(y, yt, yo + b, v);
         }
     }
 };
+
+// A thread's heads first, first + step, ... below `heads` of one token, ROPE_BATCH of them in flight.  rope_fetch may come before the
+// angles are known: what a CTA waits for longest are its first loads, and those do not depend on them.  (Two heads in flight: 24.8 and
+// 49.0 us for the rotation and the append of a prompt's chunk; one 26.0 and 54.9, four 25.5 and 51.0, eight 29.2 and 63.8, which leave fewer CTAs per SM.)
+constexpr int ROPE_BATCH = 2;
+template <int VEC>
+__device__ __forceinline__ void rope_fetch(const RopeUnit<VEC> &unit, int first, int step, int heads, int dim, const void *x, uint32_t xt, long long xo,
+                                           typename RopeUnit<VEC>::Parts (&p)[ROPE_BATCH]) {
+    if (xt == OJAS_B200_F32) {                                  // (a constant type lets the loads go out together)
+#pragma unroll
+        for (int j = 0; j < ROPE_BATCH; j++)
+            if (first + j * step < heads) unit.fetch(x, OJAS_B200_F32, xo + (long long)(first + j * step) * dim, p[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < ROPE_BATCH; j++)
+            if (first + j * step < heads) unit.fetch(x, xt, xo + (long long)(first + j * step) * dim, p[j]);
+    }
+}
+template <int VEC>
+__device__ __forceinline__ void rope_put(const RopeUnit<VEC> &unit, int first, int step, int heads, int dim, void *y, uint32_t yt, long long yo, const float2 *cs,
+                                         const typename RopeUnit<VEC>::Parts (&p)[ROPE_BATCH]) {
+#pragma unroll
+    for (int j = 0; j < ROPE_BATCH; j++)
+        if (first + j * step < heads) unit.put(p[j], y, yt, yo + (long long)(first + j * step) * dim, cs);
+}
