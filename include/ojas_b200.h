@@ -1,5 +1,6 @@
 /*
- * ojas_b200.h — C ABI of the B200 (sm_100a) quantized-matmul backend.
+ * ojas_b200.h — C ABI of the B200 (sm_100a) quantized-matmul backend, and of the rotary positions, paged cache and attention
+ * between a layer's projections.
  *
  * Every entry point takes plain pointers and sizes.  Device pointers are raw CUDA
  * device addresses (what the engine's CuBuf holds, crates/ojas-cuda/src/device.rs:20-23);

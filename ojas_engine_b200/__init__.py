@@ -1,4 +1,5 @@
-"""ojas_engine_b200 — the quantized-matmul hot path of ojas-engine, rebuilt for B200 (sm_100a).
+"""ojas_engine_b200 — the quantized-matmul hot path of ojas-engine, rebuilt for B200 (sm_100a), with the rotary positions, paged
+cache and attention between a layer's projections.
 
 The product is ``libojas_b200.so`` (CUDA kernels behind the C ABI of ``include/ojas_b200.h``);
 this package is its host-side mirror of the engine's backend interface.  There is no CPU

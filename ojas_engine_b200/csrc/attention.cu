@@ -26,7 +26,7 @@
 constexpr int AR_KEYS = 64;                                  // keys of a block
 constexpr int AR_WARPS = 4, AR_THREADS = (AR_WARPS + 1) * 32;   // consumer warps; and the producer
 constexpr int AR_STAT_BYTES = 256 + AR_WARPS * 32 * 8 + 32 * 8;   // barriers; per warp and row (maximum, sum); per row the same
-constexpr int AR_CLUSTER = 16;                               // splits that can be a cluster (above 8: allowed on this architecture when asked for)
+constexpr int AR_CLUSTER = 16;                               // most splits that can be a cluster (more than 8 have to be asked for)
 __host__ __device__ constexpr int ar_stage_bytes(int dim) { return 2 * AR_KEYS * dim * 2; }
 // 96 KB of blocks in flight per CTA, two CTAs per SM (dim 256: three 64 KB blocks, one CTA): HBM needs about 44 KB per SM and
 // microsecond of latency.
@@ -473,7 +473,7 @@ static AttnPlan attn_plan(int sm_count, size_t n_seqs, size_t M, size_t max_rows
     // (37 against 48 us for 16 f32 rows).
     p.tensor = bound > (dim == 128 && !p.two ? unit : 2 * unit);
     p.mt = bound > unit && dim <= 128 ? 2 : 1;
-    p.rows = p.tensor ? (dim == 256 || f32 ? 128 : 256) : (int)unit * p.mt;
+    p.rows = p.tensor ? (dim == 256 || f32 || bound <= 128 ? 128 : 256) : (int)unit * p.mt;
     p.block = p.tensor && dim != 256 ? 128 : 64;
     const unsigned long long by_seq = (unsigned long long)n_seqs * ((bound + p.rows - 1) / p.rows), by_row = (unsigned long long)M * group / p.rows + n_seqs;
     p.tiles = (long long)(by_seq <= by_row ? by_seq : by_row);
@@ -489,18 +489,19 @@ static AttnPlan attn_plan(int sm_count, size_t n_seqs, size_t M, size_t max_rows
     const bool pairs = dim != 256 && p.mt == 1 && !p.tensor;
     const double slots = (double)sm_count * (pairs ? 2 : 1), fixed = pairs ? 3.0 : 6.0, part = 0.5 + 0.5 / (double)n_seqs;
     const double sums = 0.25 + (double)M * (double)q_heads * (double)dim * 4.0 / 6.75e6;
+    const int largest = pairs ? AR_CLUSTER : AR_CLUSTER / 2; // with one CTA per SM sixteen would need most of a GPC at once
     double best = 0.0;
     int splits = 1;
     for (int n = 1; n <= 64 && n * 2 <= (int)blocks; n = n < 8 ? n + 1 : n + n / 4) {
         const double each = fixed + blocks / n, all = ctas * n, spread = part * all * each / slots + 0.5 * each;
-        const bool cluster = !p.tensor && n <= AR_CLUSTER && all <= slots;
+        const bool cluster = !p.tensor && n <= largest && all <= slots;
         const double cost = (all <= slots || each > spread ? each : spread) + (n == 1 ? 0.0 : cluster ? 0.1 * n : 3.0 + sums * n);
         if (n == 1 || cost < best) { best = cost; splits = n; }
     }
     p.split_blocks = (int)((blocks + splits - 1) / splits);
     p.splits = (int)(((long long)blocks + p.split_blocks - 1) / p.split_blocks);
     const size_t rows = M * q_heads;
-    p.cluster = !p.tensor && p.splits > 1 && p.splits <= AR_CLUSTER && ctas * p.splits <= slots;
+    p.cluster = !p.tensor && p.splits > 1 && p.splits <= largest && ctas * p.splits <= slots;
     p.workspace = p.splits > 1 && !p.cluster ? align256((size_t)p.splits * rows * sizeof(float2)) + (size_t)p.splits * rows * dim * sizeof(float) : 0;
     return p;
 }

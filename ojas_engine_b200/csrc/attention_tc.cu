@@ -9,8 +9,8 @@
 //   NQ = 2 (dim 64 and 128, 16-bit activations): while one tile's softmax runs the tensor cores work for the other tile.  (Blocks of
 //          64 keys would leave TMEM for probabilities beside the scores and let the scores run ahead, but every group of MMAs with a
 //          completion signal takes 300 cycles at least and N = 64 is bound by shared memory: 828 against 565 us for an 8192-token prompt.)
-//   NQ = 1 (dim 256, whose O takes half of TMEM, and f32 activations): two score buffers, whose columns the probabilities reuse;
-//          the next block's scores are formed while the softmax runs.
+//   NQ = 1 (dim 256, whose O takes half of TMEM, f32 activations, and calls of at most 128 rows per key head): two score buffers,
+//          whose columns the probabilities reuse; the next block's scores are formed while the softmax runs.
 // The accumulator is rescaled only when a row's maximum has grown by more than AT_SLACK (in log2) since it was last fixed, or a
 // block's probabilities would leave f16's range (rare after the first blocks): they are kept scaled by 2^AT_SHIFT, below
 // f16's limit and above its smallest values.
@@ -33,9 +33,10 @@ constexpr int AT_ROWS = 128;
 constexpr int AT_MAX_STAGES = 10;
 constexpr int AT_POLY = 2;                                  // of eight pairs of exponentials, those formed by the polynomial
 
-template <int D, int TERMS>
+template <int D, int TERMS, int TILES>
 struct AtShape {
-    static constexpr int NQ = D == 256 || TERMS == 2 ? 1 : 2;          // row tiles of a CTA
+    static constexpr int NQ = TILES;                                   // row tiles of a CTA
+    static_assert(NQ == 1 || (TERMS == 1 && D <= 128), "two tiles' accumulators and q");
     static constexpr int KEYS = D == 256 ? 64 : 128;                   // keys of a block
     static constexpr bool AHEAD = NQ == 1;                             // a block's scores are formed before the products of the one before
     static constexpr int STAGE = KEYS * D * 2;                         // one block of K or V
@@ -52,7 +53,7 @@ struct AtShape {
     static __host__ __device__ constexpr int col_s(int u, int n) { return NQ == 2 ? u * 128 : (n & 1) * 128; }
     static __host__ __device__ constexpr int col_o(int u) { return 256 + u * 128; }
     static constexpr int COL_SUM = 384;
-    static constexpr int CHUNK = D == 64 ? 128 : 256;                  // bytes of a row that the epilogue stages at a time
+    static constexpr int CHUNK = Q_BYTES / (SOFT_WARPS * 32) < 256 ? Q_BYTES / (SOFT_WARPS * 32) : 256;   // bytes of a row that the epilogue stages at a time
     static_assert(SOFT_WARPS * 32 * CHUNK <= Q_BYTES, "the epilogue stages rows where Q was");
     static_assert(STAGES >= 3, "a K and a V block in use and one on the way");
 };
@@ -277,10 +278,10 @@ __device__ __forceinline__ float load_q(const void *q, long long at, bool live, 
     return factor;
 }
 
-template <int D, bool BF, int TERMS>
-__global__ void __launch_bounds__(AtShape<D, TERMS>::THREADS, 1) attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k,
+template <int D, bool BF, int TERMS, int TILES>
+__global__ void __launch_bounds__(AtShape<D, TERMS, TILES>::THREADS, 1) attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k,
                                                                                   const __grid_constant__ CUtensorMap map_v, const AttnArgs a, int box_rows) {
-    using S = AtShape<D, TERMS>;
+    using S = AtShape<D, TERMS, TILES>;
     constexpr int NQ = S::NQ, KEYS = S::KEYS, STAGES = S::STAGES, STAGE = S::STAGE;
     extern __shared__ unsigned char at_raw[];
     unsigned char *smem = reinterpret_cast<unsigned char *>(((uintptr_t)at_raw + 1023) & ~(uintptr_t)1023);
@@ -528,7 +529,7 @@ __global__ void __launch_bounds__(AtShape<D, TERMS>::THREADS, 1) attn_tiles_kern
                 if (blocks == 0) asm volatile("barrier.cta.sync %0, %1;" ::"r"(9 + u), "n"(128 * S::SHARE) : "memory");   // no MMA has waited for all of Q here
                 const float by = alone ? inv : 1.0f;
                 const bool wide = !alone || a.out_stride * es % 16 == 0;
-                constexpr int PIECES = S::CHUNK / 16;        // 16-byte pieces of a row's chunk; piece p of row r lies at p ^ (r % 8)
+                constexpr int PIECES = S::CHUNK / 16, TURN = PIECES < 8 ? PIECES - 1 : 7;   // 16-byte pieces of a row's chunk; piece p of row r lies at p ^ (r & TURN)
 #pragma unroll 1
                 for (int c0 = 0; c0 < S::OUT; c0 += per) {
 #pragma unroll 1
@@ -557,11 +558,11 @@ __global__ void __launch_bounds__(AtShape<D, TERMS>::THREADS, 1) attn_tiles_kern
                         if (es == 4) {
 #pragma unroll
                             for (int i = 0; i < 8; i++)
-                                *reinterpret_cast<float4 *>(row_at + (((p0 + i) ^ (lane & 7)) << 4)) = make_float4(o[4 * i] * by, o[4 * i + 1] * by, o[4 * i + 2] * by, o[4 * i + 3] * by);
+                                *reinterpret_cast<float4 *>(row_at + (((p0 + i) ^ (lane & TURN)) << 4)) = make_float4(o[4 * i] * by, o[4 * i + 1] * by, o[4 * i + 2] * by, o[4 * i + 3] * by);
                         } else {
 #pragma unroll
                             for (int i = 0; i < 4; i++)
-                                *reinterpret_cast<uint4 *>(row_at + (((p0 + i) ^ (lane & 7)) << 4)) =
+                                *reinterpret_cast<uint4 *>(row_at + (((p0 + i) ^ (lane & TURN)) << 4)) =
                                     make_uint4(pack_half(o[8 * i] * by, o[8 * i + 1] * by, BF), pack_half(o[8 * i + 2] * by, o[8 * i + 3] * by, BF),
                                                pack_half(o[8 * i + 4] * by, o[8 * i + 5] * by, BF), pack_half(o[8 * i + 6] * by, o[8 * i + 7] * by, BF));
                         }
@@ -571,7 +572,7 @@ __global__ void __launch_bounds__(AtShape<D, TERMS>::THREADS, 1) attn_tiles_kern
                     for (int i = 0; i < PIECES; i++) {
                         const int r = (i * 32 + lane) / PIECES, p = lane % PIECES;
                         unsigned char *row_to = reinterpret_cast<unsigned char *>(__shfl_sync(0xffffffffu, (unsigned long long)to, r));
-                        const uint4 v = *reinterpret_cast<const uint4 *>(stage + r * S::CHUNK + ((p ^ (r & 7)) << 4));
+                        const uint4 v = *reinterpret_cast<const uint4 *>(stage + r * S::CHUNK + ((p ^ (r & TURN)) << 4));
                         if (row_to) {
                             uint4 *dst = reinterpret_cast<uint4 *>(row_to + c0 * es + p * 16);
                             if (wide) *dst = v;
@@ -760,11 +761,11 @@ __global__ void __launch_bounds__(AtShape<D, TERMS>::THREADS, 1) attn_tiles_kern
     }
 }
 
-template <int D, bool BF, int TERMS>
+template <int D, bool BF, int TERMS, int TILES>
 cudaError_t launch_tiles(const ojas_b200_ctx *ctx, const ojas_b200_kv *kv, const AttnArgs &a, const AttnPlan &p) {
-    using S = AtShape<D, TERMS>;
+    using S = AtShape<D, TERMS, TILES>;
     static std::atomic<uint64_t> ready{0};
-    const cudaError_t e = smem_once(ready, ctx->device, attn_tiles_kernel<D, BF, TERMS>, S::SMEM);
+    const cudaError_t e = smem_once(ready, ctx->device, attn_tiles_kernel<D, BF, TERMS, TILES>, S::SMEM);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(p.tiles * (long long)kv->heads), 1, (unsigned)p.splits);
@@ -776,11 +777,14 @@ cudaError_t launch_tiles(const ojas_b200_ctx *ctx, const ojas_b200_kv *kv, const
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = ctx->pdl ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, attn_tiles_kernel<D, BF, TERMS>, kv->map_k, kv->map_v, a, kv->box_rows);
+    return cudaLaunchKernelEx(&cfg, attn_tiles_kernel<D, BF, TERMS, TILES>, kv->map_k, kv->map_v, a, kv->box_rows);
 }
 template <bool BF, int TERMS>
 cudaError_t launch_tiles_dim(const ojas_b200_ctx *ctx, const ojas_b200_kv *kv, const AttnArgs &a, const AttnPlan &p) {
-    return kv->dim == 64 ? launch_tiles<64, BF, TERMS>(ctx, kv, a, p) : kv->dim == 128 ? launch_tiles<128, BF, TERMS>(ctx, kv, a, p) : launch_tiles<256, BF, TERMS>(ctx, kv, a, p);
+    constexpr int TWO = TERMS == 1 ? 2 : 1;
+    if (kv->dim == 64) return p.rows == 256 ? launch_tiles<64, BF, TERMS, TWO>(ctx, kv, a, p) : launch_tiles<64, BF, TERMS, 1>(ctx, kv, a, p);
+    if (kv->dim == 128) return p.rows == 256 ? launch_tiles<128, BF, TERMS, TWO>(ctx, kv, a, p) : launch_tiles<128, BF, TERMS, 1>(ctx, kv, a, p);
+    return launch_tiles<256, BF, TERMS, 1>(ctx, kv, a, p);
 }
 
 }  // namespace

@@ -301,7 +301,7 @@ class B200Gpu:
                   causal: bool = True, window: int = 0, q_stride: int = 0, out_stride: int = 0, workspace: Buf | None = None) -> None:
         """Attention of the call's rows over their sequences' keys (scale: 1 / sqrt(dim) unless given).  Without a caller
         workspace a grow-only scratch buffer owned by this object is used; a buffer it outgrew stays allocated, because a
-        captured graph may still use it."""
+        captured graph may still use it.  It grows by an allocation: make a shape's first call outside a capture."""
         if workspace is None:
             shape = (kv.heads, kv.dim, kv.page_size, kv.type, act_type, m, q_heads, window, self._ctx.value)
             need = seqs._need.get(shape)
