@@ -31,7 +31,7 @@ constexpr float AT_SHIFT = 8.0f, AT_SLACK = 7.0f;
 constexpr float AT_SUM_MOST = 49152.0f;                    // (a block of 128 scores at the maximum gives 128 * 2^AT_SHIFT = 32768)
 constexpr int AT_ROWS = 128;
 constexpr int AT_MAX_STAGES = 10;
-constexpr int AT_POLY = 2;                                  // of eight pairs of exponentials, those formed by the polynomial
+constexpr int AT_POLY = 1;                                  // of eight pairs of exponentials, those formed by the polynomial
 
 template <int D, int TERMS, int TILES>
 struct AtShape {
