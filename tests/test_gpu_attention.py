@@ -521,3 +521,19 @@ def test_two_streams_at_once(gpu):
         o.sync()
         check(out, want, attention_bound(want, weight, vmax, 128, 9000, F32, F16, 2))
         o.close()
+
+
+@pytest.mark.parametrize("rows", [1, 3, 30, 150])
+def test_without_overlapping_launches(rows):
+    """Option pdl = 0: the same results, every kernel waiting for the one before; the profiler names them."""
+    g = ob.B200Gpu(0)
+    b = Batch([rows, 1], [5000, 90], kv_heads=2, dim=128, seed=5)
+    b.upload(g)
+    first = run_attention(g, b, 8, F32)
+    g.set_option("pdl", 0)
+    g.set_option("profile", 1)
+    again = run_attention(g, b, 8, F32)
+    names = {name for name, _, _ in g.profile_report()}
+    assert names and names <= {"attn_rows", "attn_tiles", "attn_join"}
+    assert torch.equal(first, again)
+    g.close()
