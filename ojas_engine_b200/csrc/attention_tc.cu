@@ -109,11 +109,13 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // 2^y of two values on the multiply-add units: y = j + f, |f| <= 1/2, 2^f by a polynomial of degree 4 (least largest relative error
 // on that interval, 2.7e-6; P is rounded to 2^-12 or more), j added to the exponent.  The special-function unit gives 16 exponentials
 // a cycle per SM, as long for a tile's scores as the tensor cores need for both its products: a part is formed here instead.
-// Below 2^-126 the result is about 2^-126.
+// Below 2^-126 the result is zero; above 2^127, and for NaN, it is 2^127, which no sum that is kept holds.
 __device__ __forceinline__ void exp2_poly(uint64_t y, float &p0, float &p1) {
     float a, b;
     unpair(y, a, b);
-    y = pair(fmaxf(a, -126.0f), fmaxf(b, -126.0f));
+    a = fminf(a, 127.0f);                                    // (the smaller of NaN and a number is the number)
+    b = fminf(b, 127.0f);
+    y = pair(a, b);
     const uint64_t magic = pair(12582912.0f, 12582912.0f), unmagic = pair(-12582912.0f, -12582912.0f);   // 1.5 * 2^23: rounds to whole numbers
     const uint64_t r = add2(y, magic), f = fma2(add2(r, unmagic), pair(-1.0f, -1.0f), y);
     uint64_t p = fma2(pair(0.009570101276040077f, 0.009570101276040077f), f, pair(0.05591785907745361f, 0.05591785907745361f));
@@ -123,8 +125,8 @@ __device__ __forceinline__ void exp2_poly(uint64_t y, float &p0, float &p1) {
     float r0, r1;
     unpair(p, p0, p1);
     unpair(r, r0, r1);
-    p0 = __int_as_float(__float_as_int(p0) + (__float_as_int(r0) << 23));
-    p1 = __int_as_float(__float_as_int(p1) + (__float_as_int(r1) << 23));
+    p0 = a < -126.0f ? 0.0f : __int_as_float(__float_as_int(p0) + (__float_as_int(r0) << 23));
+    p1 = b < -126.0f ? 0.0f : __int_as_float(__float_as_int(p1) + (__float_as_int(r1) << 23));
 }
 
 // Bounded wait without a call (ptxas splits registers between the roles only in code without calls).  Whole warps or one thread.

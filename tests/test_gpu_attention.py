@@ -537,3 +537,32 @@ def test_without_overlapping_launches(rows):
     assert names and names <= {"attn_rows", "attn_tiles", "attn_join"}
     assert torch.equal(first, again)
     g.close()
+
+
+@pytest.mark.parametrize("act,cache", TYPES)
+@pytest.mark.parametrize("dim,rows", [(128, 100), (64, 40), (128, 2), (256, 90)])
+def test_one_key_far_above_or_below_the_others(gpu, act, cache, dim, rows):
+    """A key of the second or third hundred, in sequence c the one at 128 + c, whose scores differ from all others by hundreds, up or
+    down: more than an f32 exponent holds, at every place of a block."""
+    b = Batch([rows] * 128, [300 + rows] * 128, kv_heads=1, dim=dim, page=64, cache=cache, seed=dim + rows)
+    for c, k in enumerate(b.k_rows):
+        k[128 + c] *= 200.0
+        b.put(b.k, c, 0, k)
+    b.upload(gpu)
+    run_attention(gpu, b, 2, act)
+
+
+@pytest.mark.parametrize("act,cache", TYPES)
+@pytest.mark.parametrize("dim,rows", [(128, 100), (64, 40), (128, 2), (256, 90)])
+def test_a_key_of_nan_reaches_every_row_that_sees_it(gpu, act, cache, dim, rows):
+    b = Batch([rows] * 128, [300 + rows] * 128, kv_heads=2, dim=dim, page=64, cache=cache, seed=dim + rows)
+    for c, k in enumerate(b.k_rows):
+        k[128 + c, 1, 7] = math.nan
+        b.put(b.k, c, 0, k)
+    b.upload(gpu)
+    q = randn(torch.Generator().manual_seed(4), b.M, 4, dim).to(TORCH[act]).cuda()
+    out = torch.empty_like(q)
+    torch.cuda.synchronize()
+    gpu.attention(b.kv, b.seqs, buf(q), buf(out), b.M, 4, act_type=act)
+    gpu.sync()
+    assert out[:, 2:].isnan().all() and out[:, :2].isfinite().all()
