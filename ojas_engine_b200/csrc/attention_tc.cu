@@ -31,7 +31,6 @@ constexpr float AT_SHIFT = 8.0f, AT_SLACK = 7.0f;
 constexpr float AT_SUM_MOST = 49152.0f;                    // (a block of 128 scores at the maximum gives 128 * 2^AT_SHIFT = 32768)
 constexpr int AT_ROWS = 128;
 constexpr int AT_MAX_STAGES = 10;
-constexpr int AT_POLY = 1;                                  // of eight pairs of exponentials, those formed by the polynomial
 
 template <int D, int TERMS, int TILES>
 struct AtShape {
@@ -106,29 +105,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
-// 2^y of two values on the multiply-add units: y = j + f, |f| <= 1/2, 2^f by a polynomial of degree 4 (least largest relative error
-// on that interval, 2.7e-6; P is rounded to 2^-12 or more), j added to the exponent.  The special-function unit gives 16 exponentials
-// a cycle per SM, as long for a tile's scores as the tensor cores need for both its products: a part is formed here instead.
-// Below 2^-126 the result is zero; above 2^127, and for NaN, it is 2^127, which no sum that is kept holds.
-__device__ __forceinline__ void exp2_poly(uint64_t y, float &p0, float &p1) {
-    float a, b;
-    unpair(y, a, b);
-    a = fminf(a, 127.0f);                                    // (the smaller of NaN and a number is the number)
-    b = fminf(b, 127.0f);
-    y = pair(a, b);
-    const uint64_t magic = pair(12582912.0f, 12582912.0f), unmagic = pair(-12582912.0f, -12582912.0f);   // 1.5 * 2^23: rounds to whole numbers
-    const uint64_t r = add2(y, magic), f = fma2(add2(r, unmagic), pair(-1.0f, -1.0f), y);
-    uint64_t p = fma2(pair(0.009570101276040077f, 0.009570101276040077f), f, pair(0.05591785907745361f, 0.05591785907745361f));
-    p = fma2(p, f, pair(0.240247443318367f, 0.240247443318367f));
-    p = fma2(p, f, pair(0.6931217908859253f, 0.6931217908859253f));
-    p = fma2(p, f, pair(0.9999992847442627f, 0.9999992847442627f));
-    float r0, r1;
-    unpair(p, p0, p1);
-    unpair(r, r0, r1);
-    p0 = a < -126.0f ? 0.0f : __int_as_float(__float_as_int(p0) + (__float_as_int(r0) << 23));
-    p1 = b < -126.0f ? 0.0f : __int_as_float(__float_as_int(p1) + (__float_as_int(r1) << 23));
-}
-
 // Bounded wait without a call (ptxas splits registers between the roles only in code without calls).  Whole warps or one thread.
 __device__ __forceinline__ bool at_wait(uint64_t *bar, uint32_t parity, volatile int *abort_flag, unsigned *status) {
     if (mbar_test(bar, parity)) return true;
@@ -393,7 +369,15 @@ __global__ void __launch_bounds__(AtShape<D, TERMS, TILES>::THREADS, 1) attn_til
             // Most blocks raise no row's maximum by much: their probabilities are formed against the maximum so far, without looking
             // for the block's own, and kept if their sum, and with it each of them, is in f16's range (NaN is not).
             const bool edge = live && (blk * KEYS < see_lo || (blk + 1) * KEYS > see_hi);
-            bool again = __any_sync(0xffffffffu, !ok || edge || (live && m == -INFINITY));
+            if (__any_sync(0xffffffffu, edge)) {
+#pragma unroll
+                for (int c = 0; c < S::COLS; c += 32) {      // a bit for each of 32 keys that the row sees
+                    const uint32_t seen = below(see_hi - key0 - c) & ~below(see_lo - key0 - c);
+#pragma unroll
+                    for (int i = 0; i < 32; i++) x[c + i] = seen >> i & 1u ? x[c + i] : -INFINITY;
+                }
+            }
+            bool again = __any_sync(0xffffffffu, !ok || (live && m == -INFINITY));
             float more = 0.0f, slack = AT_SLACK;
             // The probabilities overwrite scores: not before the other thread of the row has read its own.
             if (S::SHARE == 2) pair_sync(pair_bar);
@@ -408,13 +392,9 @@ __global__ void __launch_bounds__(AtShape<D, TERMS, TILES>::THREADS, 1) attn_til
                         const float x0 = x[c + 2 * i], x1 = x[c + 2 * i + 1];
                         const uint64_t y = fma2(pair(x0, x1), by, less);
                         float p0, p1;
-                        if (TERMS == 1 && i % 8 < AT_POLY) {
-                            exp2_poly(y, p0, p1);
-                        } else {
-                            unpair(y, p0, p1);
-                            p0 = exp2_fast(p0);
-                            p1 = exp2_fast(p1);
-                        }
+                        unpair(y, p0, p1);
+                        p0 = exp2_fast(p0);
+                        p1 = exp2_fast(p1);
                         sum[i & 1] = add2(sum[i & 1], pair(p0, p1));
                         if (TERMS == 2) split_two<BF>(p0, p1, p16[i], lo16[i]);
                         else p16[i] = pack_half(p0, p1, BF);
@@ -431,14 +411,6 @@ __global__ void __launch_bounds__(AtShape<D, TERMS, TILES>::THREADS, 1) attn_til
             if (S::SHARE == 2) again = pair_any(pair_bar, again);
             if (again) {
                 at_wait_st();                                // what a failed attempt stored is stored again
-                if (edge) {
-#pragma unroll
-                    for (int c = 0; c < S::COLS; c += 32) {  // a bit for each of 32 keys that the row sees
-                        const uint32_t seen = below(see_hi - key0 - c) & ~below(see_lo - key0 - c);
-#pragma unroll
-                        for (int i = 0; i < 32; i++) x[c + i] = seen >> i & 1u ? x[c + i] : -INFINITY;
-                    }
-                }
                 float tops[4];                               // four chains: one would be COLS dependent steps
 #pragma unroll
                 for (int c = 0; c < 4; c++) tops[c] = fmaxf(x[c], x[c + 4]);
