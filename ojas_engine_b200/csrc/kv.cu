@@ -136,7 +136,7 @@ struct AppendArgs {
 // One CTA per token, as rope_rows: the first loads of q, k and v go out before the token's place is looked up.
 template <int VEC>
 __global__ void __launch_bounds__(256) kv_append_kernel(const AppendArgs a) {
-    extern __shared__ float2 append_cs[];                // [rot / 2]
+    extern __shared__ float4 append_cs[];                // (cos, sin) of two pairs each
     __shared__ long long row_at_s;                       // element offset of the token's row of head 0 in the cache; -1: not written
     __shared__ int row_pos_s;                            // position of rotation
     __shared__ bool row_live_s;                          // the row belongs to a sequence
@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const AppendArgs a) {
     }
     __syncthreads();
     if (!row_live_s) return;
-    for (int f = threadIdx.x; f < rot >> 1; f += blockDim.x) append_cs[f] = rope_angle(row_pos_s, __ldg(a.turns + f), a.magnitude);
+    for (int f = threadIdx.x; f < rot >> 1; f += blockDim.x) reinterpret_cast<float2 *>(append_cs)[f] = rope_angle(row_pos_s, __ldg(a.turns + f), a.magnitude);
     __syncthreads();
     const long long row_at = row_at_s, q_to = t * a.q_out_stride;
     if (row_at >= 0) {
@@ -253,7 +253,7 @@ extern "C" int ojas_b200_kv_append(ojas_b200_ctx *ctx, const ojas_b200_kv *kv, c
     a.q_heads = (int)q_heads; a.kv_heads = (int)kv->heads; a.dim = (int)kv->dim;
     const bool vec = rope_vec_ok(a.rot, a.dim, a.interleaved) && rope_rows_aligned(k, x_type, a.k_stride) && rope_rows_aligned(v, x_type, a.v_stride) &&
                      (q_heads == 0 || (rope_rows_aligned(q, x_type, a.q_stride) && rope_rows_aligned(q_out, q_type, a.q_out_stride)));
-    const size_t smem = (size_t)(a.rot / 2) * sizeof(float2);
+    const size_t smem = (size_t)((a.rot / 2 + 1) / 2) * sizeof(float4);
     DeviceGuard guard(ctx->device);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)M); cfg.blockDim = dim3(256); cfg.dynamicSmemBytes = smem; cfg.stream = ctx->stream;

@@ -96,7 +96,7 @@ struct RopeArgs {
 // unit of a head (VEC pairs, or 2 VEC elements that pass through) and walks the heads.  HBM bound: x in, y out.
 template <int VEC>
 __global__ void __launch_bounds__(256) rope_rows_kernel(const RopeArgs a) {
-    extern __shared__ float2 rope_cs[];           // [rot / 2]
+    extern __shared__ float4 rope_cs[];           // (cos, sin) of two pairs each
     grid_launch_dependents();
     grid_dependency_wait();                       // x and pos come from the kernels before this one
     const long long t = blockIdx.x, xo = t * a.x_stride, yo = t * a.y_stride;
@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(256) rope_rows_kernel(const RopeArgs a) {
     typename RopeUnit<VEC>::Parts p[ROPE_BATCH];
     const int pos = __ldg(a.pos + t);
     rope_fetch(unit, ty, ny, a.heads, a.dim, a.x, a.x_type, xo, p);
-    for (int f = ty * blockDim.x + threadIdx.x; f < a.rot >> 1; f += ny * blockDim.x) rope_cs[f] = rope_angle(pos, __ldg(a.turns + f), a.magnitude);
+    for (int f = ty * blockDim.x + threadIdx.x; f < a.rot >> 1; f += ny * blockDim.x) reinterpret_cast<float2 *>(rope_cs)[f] = rope_angle(pos, __ldg(a.turns + f), a.magnitude);
     __syncthreads();
     rope_put(unit, ty, ny, a.heads, a.dim, a.y, a.y_type, yo, rope_cs, p);
     for (int u = threadIdx.x; u < units; u += blockDim.x) {
@@ -135,7 +135,7 @@ extern "C" int ojas_b200_rope_rows(ojas_b200_ctx *ctx, const ojas_b200_rope *rop
     const bool vec = rope_vec_ok(a.rot, a.dim, a.interleaved) && rope_rows_aligned(x, x_type, a.x_stride) && rope_rows_aligned(y, y_type, a.y_stride);
     const int units = rope_units(vec ? 4 : 1, a.rot, a.dim);
     const dim3 block(units < 256 ? units : 256, units < 256 ? 256 / units : 1);
-    const size_t smem = (size_t)(a.rot / 2) * sizeof(float2);
+    const size_t smem = (size_t)((a.rot / 2 + 1) / 2) * sizeof(float4);
     DeviceGuard guard(ctx->device);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)M); cfg.blockDim = block; cfg.dynamicSmemBytes = smem; cfg.stream = ctx->stream;

@@ -61,7 +61,8 @@ struct RopeUnit {
             p.b.x = load_elem(x, xt, xo + b);
         }
     }
-    __device__ __forceinline__ void put(const Parts &in, void *y, uint32_t yt, long long yo, const float2 *cs) const {
+    // angles: (cos, sin) of two pairs each, so that their type asks for the alignment with which they are read.
+    __device__ __forceinline__ void put(const Parts &in, void *y, uint32_t yt, long long yo, const float4 *angles) const {
         if (f == -2) return;
         const float4 p = in.a, q = in.b;
         if (VEC == 4) {
@@ -71,7 +72,7 @@ struct RopeUnit {
                 return;
             }
             // (cos, sin) of two frequencies each: pairs 0, 1 and 2, 3 of the unit
-            const float4 c01 = *reinterpret_cast<const float4 *>(cs + f), c23 = *reinterpret_cast<const float4 *>(cs + (inter ? f2 : f + 2));
+            const float4 c01 = angles[f >> 1], c23 = angles[inter ? f2 >> 1 : (f >> 1) + 1];
             float4 u, v;
             if (inter) {                                        // p = pairs 0, 1; q = pairs 2, 3
                 u = make_float4(p.x * c01.x - p.y * c01.y, p.y * c01.x + p.x * c01.y, p.z * c01.z - p.w * c01.w, p.w * c01.z + p.z * c01.w);
@@ -85,7 +86,7 @@ struct RopeUnit {
         } else {
             float u = p.x, v = q.x;
             if (f >= 0) {
-                const float2 c = cs[f];
+                const float2 c = reinterpret_cast<const float2 *>(angles)[f];
                 u = p.x * c.x - q.x * c.y;
                 v = q.x * c.x + p.x * c.y;
             }
@@ -113,9 +114,9 @@ __device__ __forceinline__ void rope_fetch(const RopeUnit<VEC> &unit, int first,
     }
 }
 template <int VEC>
-__device__ __forceinline__ void rope_put(const RopeUnit<VEC> &unit, int first, int step, int heads, int dim, void *y, uint32_t yt, long long yo, const float2 *cs,
+__device__ __forceinline__ void rope_put(const RopeUnit<VEC> &unit, int first, int step, int heads, int dim, void *y, uint32_t yt, long long yo, const float4 *angles,
                                          const typename RopeUnit<VEC>::Parts (&p)[ROPE_BATCH]) {
 #pragma unroll
     for (int j = 0; j < ROPE_BATCH; j++)
-        if (first + j * step < heads) unit.put(p[j], y, yt, yo + (long long)(first + j * step) * dim, cs);
+        if (first + j * step < heads) unit.put(p[j], y, yt, yo + (long long)(first + j * step) * dim, angles);
 }
