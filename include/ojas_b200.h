@@ -328,7 +328,8 @@ OJAS_B200_API void ojas_b200_kv_destroy(ojas_b200_kv *kv);
  * bounds on the new rows and the length of any sequence: kernels are chosen and split by them.  Entries of the table are
  * read only for tokens that are needed (under a window, entries in front of it may be anything).
  * A description that leads outside the cache or the call touches no memory there: such a token is not appended, such a key
- * reads as zeros, rows beyond max_rows may be left out, and ojas_b200_sync returns OJAS_B200_E_DEVICE. */
+ * reads as zeros, rows inside the call keep the places that cu[b + 1] and len[b] give them, rows beyond max_rows or of offsets
+ * that go back may be left out or hold anything, and ojas_b200_sync returns OJAS_B200_E_DEVICE. */
 typedef struct {
     const int32_t *cu;          /* [n_seqs + 1] */
     const int32_t *len;         /* [n_seqs] */

@@ -30,24 +30,30 @@ struct RowTile {
     int len;                             // keys that may be read
 };
 
-// First row and number of rows of sequence s, clamped to the call.
-__device__ __forceinline__ void seq_rows(const BatchArgs &b, int s, int &first, int &n) {
-    first = max(0, __ldg(b.cu + s));
-    n = (int)max(0ll, min((long long)__ldg(b.cu + s + 1), b.M) - first);
+// First row and number of rows of sequence s, clamped to the call, and its end as given.  False: its offsets lead outside the call, or back.
+__device__ __forceinline__ bool seq_rows(const BatchArgs &b, int s, int &first, int &n, int &end) {
+    const int start = __ldg(b.cu + s);
+    end = __ldg(b.cu + s + 1);
+    first = max(0, start);
+    n = (int)max(0ll, min((long long)end, b.M) - first);
+    return seq_in_call(start, end, b.M);
 }
 
 // One warp, all lanes: which rows tile `tile` of the call is.  With per_seq > 0 every sequence has that many tiles, used or not; else
 // tiles are counted over the sequences' rows, 128 sequences at a time.  False: no such rows.  Every value is clamped so that no
-// description, however wrong, leads outside the arrays; a wrong one sets the status bit.
+// description, however wrong, leads outside the arrays; a wrong one sets the status bit.  (Every sequence is looked at by some tile: with
+// per_seq by its own; else the offsets in front of the first wrong ones hold fewer tiles than the call has, so its last tile looks past them.)
 __device__ __forceinline__ bool find_tile(const AttnArgs &a, int tile, int rows, int lane, RowTile &t) {
     const BatchArgs &b = a.batch;
-    int first = 0, n = 0;
+    int first = 0, n = 0, end = 0;
+    bool in_call = true;
     long long before = 0;                                         // tiles of the sequences in front
     if (a.per_seq > 0) {
         t.seq = tile / a.per_seq;
         if (t.seq >= b.n_seqs) return false;
         before = (long long)t.seq * a.per_seq;
-        seq_rows(b, t.seq, first, n);
+        in_call = seq_rows(b, t.seq, first, n, end);
+        if (!in_call && lane == 0) atomicOr(b.status, OJAS_ST_BATCH);
     } else {
         bool found = false;
         for (int s0 = 0; s0 < b.n_seqs && !found; s0 += 128) {
@@ -56,7 +62,7 @@ __device__ __forceinline__ bool find_tile(const AttnArgs &a, int tile, int rows,
             for (int i = 0; i < 4; i++) {
                 const int s = s0 + lane * 4 + i;
                 start[i] = count[i] = 0;
-                if (s < b.n_seqs) seq_rows(b, s, start[i], count[i]);
+                if (s < b.n_seqs && !seq_rows(b, s, start[i], count[i], end)) in_call = false;
                 tiles[i] = (int)(((long long)count[i] * a.group + rows - 1) / rows);
                 sum += tiles[i];
             }
@@ -83,14 +89,16 @@ __device__ __forceinline__ bool find_tile(const AttnArgs &a, int tile, int rows,
                 before += __shfl_sync(0xffffffffu, upto, 31);
             }
         }
+        if (!in_call) atomicOr(b.status, OJAS_ST_BATCH);
         if (!found) return false;
+        end = __ldg(b.cu + t.seq + 1);
     }
     t.token0 = first;
     t.n_rows = n * a.group;
     t.row0 = (int)(tile - before) * rows;
     const int len = __ldg(b.len + t.seq);
     const long long room = (long long)b.table_stride * b.page_size;
-    t.pos0 = len - n;
+    t.pos0 = (int)max(-0x40000000ll, min(0x7fffffffll, (long long)len - end + first));   // where the append puts the row, whatever lies outside the call
     t.len = (int)max(0ll, min((long long)len, room));
     if (lane == 0 && n > 0 && ((long long)len > room || len < n || n > b.max_rows)) atomicOr(b.status, OJAS_ST_BATCH);
     return t.row0 >= 0 && t.row0 < t.n_rows;                      // (offsets out of order could overflow the count)

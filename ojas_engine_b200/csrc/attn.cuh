@@ -89,6 +89,8 @@ __device__ __forceinline__ void store_elem4(void *p, uint32_t type, long long i,
 }
 
 // ---------------------------------------------------------------------------- which sequence a row belongs to
+// Rows [start, end) of a sequence lie in a call of M rows.
+__device__ __forceinline__ bool seq_in_call(int start, int end, long long M) { return start >= 0 && end >= start && end <= M; }
 // One warp, all lanes together: the sequence b with cu[b] <= row < cu[b + 1], or -1.  Each step narrows the range by 32.
 // Out-of-order offsets give some sequence or -1, never an index outside the batch.
 __device__ __forceinline__ int find_seq(const int *cu, int n_seqs, long long row, int lane) {

@@ -174,6 +174,11 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const AppendArgs a) {
             row_pos_s = pos;
         }
     }
+    // The second warp looks at the offsets themselves, a share of them per CTA: rows outside the call have no CTA of their own.
+    if (threadIdx.x >> 5 == 1) {
+        for (long long b = t * 32 + lane; b < a.batch.n_seqs; b += a.batch.M * 32)
+            if (!seq_in_call(__ldg(a.batch.cu + b), __ldg(a.batch.cu + b + 1), a.batch.M)) atomicOr(a.batch.status, OJAS_ST_BATCH);
+    }
     __syncthreads();
     if (!row_live_s) return;
     for (int f = threadIdx.x; f < rot >> 1; f += blockDim.x) reinterpret_cast<float2 *>(append_cs)[f] = rope_angle(row_pos_s, __ldg(a.turns + f), a.magnitude);

@@ -3,7 +3,7 @@ import pytest
 import torch
 
 import ojas_engine_b200 as ob
-from attn_helpers import TORCH, Batch, buf, check, rope_bound, rope_exact
+from attn_helpers import TORCH, Batch, attention_bound, buf, check, rope_bound, rope_exact
 
 pytestmark = pytest.mark.gpu
 F32, F16, BF16 = ob.F32, ob.F16, ob.BF16
@@ -37,3 +37,56 @@ def test_append_head_sizes(gpu, layout, xt, ct, qt, dim, rot, hq, hk):
             want = rope_exact(part, pos, freq, layout)
             check(got, want, rope_bound(part, want, rot, layout, 1.0, t))
         assert torch.equal(vc[at], rows[:, hq + hk :].to(TORCH[ct]))
+
+
+# ------------------------------------------------------------------------------------------ rows outside the call
+@pytest.mark.parametrize("shift,cut", [(0, 2), (0, 5), (0, 6), (-1, 0), (-4, 0)])
+@pytest.mark.parametrize("rows,max_rows", [([3, 2, 5], 5), ([40, 30, 5], 40), ([1] * 140 + [5], 5), ([1] * 140 + [5], 600)])
+def test_rows_outside_the_call_are_reported(gpu, rows, max_rows, shift, cut):
+    """Offsets that lead behind the call's last row (``cut`` rows, the last sequence wholly among them from five on) or in front of its
+    first: an error from either call; the rows inside are stored and attended at the places their sequences give them.  Row tiles
+    of every sequence (max_rows near the rows) and tiles counted over the sequences."""
+    b = Batch(rows, [n + 20 for n in rows], kv_heads=1, dim=64, seed=3, max_rows=max_rows)
+    q, total = randn(1, b.M, 4, 64), b.M
+    want, weight, vmax = b.attention_exact(q, 4)
+    bound = attention_bound(want, weight, vmax, 64, max(b.lens), F32, F16, 2)
+    b.cu += shift
+    b.upload(gpu)
+    m = total + shift - cut                                    # rows of the call: those of q from -shift on
+    inside = slice(-shift, -shift + m)
+    qd, out = q[inside].contiguous().cuda(), torch.full((m + 3, 4, 64), 77.0).cuda()
+    torch.cuda.synchronize()
+    gpu.attention(b.kv, b.seqs, buf(qd), buf(out), m, 4)
+    with pytest.raises(ob.OjasB200Error) as e:
+        gpu.sync()
+    assert e.value.code == -5 and "batch" in str(e.value)
+    torch.cuda.synchronize()
+    check(out[:m], want[inside], bound[inside])
+    assert (out[m:] == 77).all()
+    x, before = randn(2, m, 64).cuda(), b.dev["k"].clone()
+    torch.cuda.synchronize()
+    gpu.kv_append(b.kv, b.seqs, buf(x), buf(x), m)
+    with pytest.raises(ob.OjasB200Error) as e:
+        gpu.sync()
+    assert e.value.code == -5 and "batch" in str(e.value)
+    torch.cuda.synchronize()
+    t, stored, old = 0, b.view(b.dev["k"].cpu()), b.view(before.cpu())
+    for i, (n, length) in enumerate(zip(b.rows, b.lens)):
+        for p in range(length - n, length):
+            row, at = t + shift, (b.table[i, p // b.page], p % b.page)
+            t += 1
+            kept = row < 0 or row >= m or int(b.cu[i]) < 0     # (a sequence that begins in front of the call is not stored)
+            assert torch.equal(stored[at][0], old[at][0] if kept else x[row].half().cpu()), (i, p)
+            old[at] = stored[at]
+    assert torch.equal(stored.nan_to_num(nan=9.0), old.nan_to_num(nan=9.0))
+
+
+def test_a_batch_with_nothing_wrong_is_not_reported(gpu):
+    """Empty sequences at both ends, rows behind the last one, fewer rows than the call has."""
+    b = Batch([0, 3, 0, 1, 0], [0, 40, 7, 9, 0], kv_heads=1, dim=64, seed=3, extra_rows=4, max_rows=300).upload(gpu)
+    q = randn(1, b.M, 4, 64).cuda()
+    out = torch.empty_like(q)
+    torch.cuda.synchronize()
+    gpu.attention(b.kv, b.seqs, buf(q), buf(out), b.M, 4)
+    gpu.kv_append(b.kv, b.seqs, buf(q), buf(q), b.M, x_stride=256)
+    gpu.sync()
