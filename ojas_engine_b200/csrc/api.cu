@@ -319,8 +319,9 @@ extern "C" int ojas_b200_sync(ojas_b200_ctx *ctx) {
     const unsigned int st = *(volatile unsigned int *)ctx->host_status;
     if (st != 0) {
         *(volatile unsigned int *)ctx->host_status = 0;
-        if (st == 0x100000u) return ojas_fail(ctx, OJAS_B200_E_DEVICE, "a page number, a length or a row range of a batch lies outside its cache or call (status word 0x%x)", st);
-        return ojas_fail(ctx, OJAS_B200_E_DEVICE, "a kernel gave up a bounded wait (status word 0x%x)", st);
+        const bool batch = (st & OJAS_ST_BATCH) != 0, wait = (st & ~OJAS_ST_BATCH) != 0;
+        return ojas_fail(ctx, OJAS_B200_E_DEVICE, "%s%s%s (status word 0x%x)", batch ? "a page number, a length or a row range of a batch lies outside its cache or call" : "",
+                         batch && wait ? "; " : "", wait ? "a kernel gave up a bounded wait" : "", st);
     }
     return 0;
 }

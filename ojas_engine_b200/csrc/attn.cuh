@@ -6,10 +6,6 @@
 
 #include "common.cuh"
 
-// Bits of the context's status word set by these kernels (ojas_b200_sync turns them into OJAS_B200_E_DEVICE).
-constexpr unsigned OJAS_ST_BATCH = 0x100000u;      // a page number, a length or a row range outside the cache or the call
-constexpr unsigned OJAS_ST_ATTN_WAIT = 0x200000u;  // a bounded wait of an attention kernel ran out
-
 // Rotation of one pair per frequency.  turns[i] is the frequency in turns per position as a 64-bit binary fraction, so
 // pos * turns[i] modulo 2^64 is the pair's angle modulo one turn, exactly, for every 32-bit position.
 struct ojas_b200_rope {

@@ -46,6 +46,17 @@ constexpr size_t OJAS_ACT_SCRATCH_VALUES = 262144;
 constexpr size_t OJAS_ACT_SCRATCH_BYTES = (size_t)1 << 20;
 static_assert(OJAS_ACT_SCRATCH_VALUES + OJAS_ACT_SCRATCH_VALUES / 256 * 4 + OJAS_ACT_SCRATCH_VALUES / 32 * 4 <= OJAS_ACT_SCRATCH_BYTES, "Q8_K scratch");
 
+// Bits of the context's status word (ojas_b200_sync turns it into OJAS_B200_E_DEVICE).  Each is set at one place, by the wait there that
+// ran out, except for the one that says that a caller's batch was wrong.
+constexpr unsigned OJAS_ST_GEMV_WAIT = 0x40u;           // gemv.cu
+constexpr unsigned OJAS_ST_GEMM_WAITS = 0x3ff00u;       // gemm_ts.cuh
+constexpr unsigned OJAS_ST_JOIN_WAIT = 0x80000u;        // tp.cu
+constexpr unsigned OJAS_ST_EXPERT_WAITS = 0x1fd00000u;  // experts_i8.cu
+constexpr unsigned OJAS_ST_ATTN_WAIT = 0x200000u;       // attention.cu, attention_tc.cu
+constexpr unsigned OJAS_ST_BATCH = 0x20000000u;         // a page number, a length or a row range outside the cache or the call
+static_assert((OJAS_ST_GEMV_WAIT | OJAS_ST_GEMM_WAITS | OJAS_ST_JOIN_WAIT | OJAS_ST_EXPERT_WAITS | OJAS_ST_ATTN_WAIT | OJAS_ST_BATCH) ==
+                  OJAS_ST_GEMV_WAIT + OJAS_ST_GEMM_WAITS + OJAS_ST_JOIN_WAIT + OJAS_ST_EXPERT_WAITS + OJAS_ST_ATTN_WAIT + OJAS_ST_BATCH, "a status bit with two meanings");
+
 int ojas_fail(ojas_b200_ctx *ctx, int code, const char *fmt, ...);
 
 #define OJAS_CUDA(ctx, call)                                                                     \

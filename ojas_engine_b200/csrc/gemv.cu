@@ -118,7 +118,7 @@ __device__ __forceinline__ void gv_bar_wait(uint64_t *bar, unsigned parity, unsi
         if (gv_bar_try(bar, parity)) return;
     if (!dead) {
         dead = true;
-        atomicOr(status, 0x40u);
+        atomicOr(status, OJAS_ST_GEMV_WAIT);
         __threadfence_system();
     }
 }

@@ -242,7 +242,7 @@ __global__ void __launch_bounds__(256) tp_join_kernel(const TpJoinArgs a) {
     // a rank did not deliver in time: report (y keeps what it had there), and still finish the step so that the context stays usable
     const int bad = __syncthreads_or(ok ? 0 : 1);
     if (threadIdx.x == 0) {
-        if (bad) { atomicOr(a.status, 0x80000u); __threadfence_system(); }
+        if (bad) { atomicOr(a.status, OJAS_ST_JOIN_WAIT); __threadfence_system(); }
         __threadfence();
         const unsigned old = atomicAdd(a.joined, 1u);
         if (old == gridDim.x - 1) {          // the block that finishes last closes the step

@@ -3,6 +3,7 @@ import pytest
 import torch
 
 import ojas_engine_b200 as ob
+from ojas_engine_b200 import tp
 from attn_helpers import TORCH, Batch, attention_bound, buf, check, rope_bound, rope_exact
 
 pytestmark = pytest.mark.gpu
@@ -90,3 +91,24 @@ def test_a_batch_with_nothing_wrong_is_not_reported(gpu):
     gpu.attention(b.kv, b.seqs, buf(q), buf(out), b.M, 4)
     gpu.kv_append(b.kv, b.seqs, buf(q), buf(q), b.M, x_stride=256)
     gpu.sync()
+
+
+def test_a_wrong_batch_and_a_lost_wait_are_both_named(gpu):
+    """One status word for two errors: the message says both, and after each alone only that one."""
+    b = Batch([1], [20], kv_heads=1, dim=64, seed=3).upload(gpu)
+    b.dev["table"][0, 0] = b.pages
+    q = randn(1, 1, 4, 64).cuda()
+    out, y = torch.empty_like(q), gpu.alloc(64)
+    group = tp.TpGroup(gpu, 1, 0, 64, lambda blob: [blob])
+    group.set_wait_us(2000)
+    torch.cuda.synchronize()
+    for batch, wait in ((True, True), (True, False), (False, True)):
+        if batch:
+            gpu.attention(b.kv, b.seqs, buf(q), buf(out), 1, 4)
+        if wait:
+            group.join(group.COL, y, 64)                      # nothing was pushed: its wait ends by itself
+        with pytest.raises(ob.OjasB200Error) as e:
+            gpu.sync()
+        assert ("batch" in str(e.value)) == batch and ("bounded wait" in str(e.value)) == wait
+    group.close()
+    gpu.free(y)
