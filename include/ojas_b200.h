@@ -301,8 +301,9 @@ OJAS_B200_API void ojas_b200_rope_destroy(ojas_b200_rope *rope);
 OJAS_B200_API int ojas_b200_rope_frequencies(size_t rot_dim, double base, const ojas_b200_rope_scaling *scaling, const float *freq_factors,
                                              double *radians_out, char *err, size_t errlen);
 /* y[m, h, :] = x[m, h, :] with the first rot_dim elements turned by position pos[m] (device, any int32, negative ones turn
- * back).  layout: pairs are (i, i + rot_dim / 2) (half) or (2i, 2i + 1) (interleaved).  dim even, at most 2048.  Angles are exact
- * to 2e-9 radians at every position.  x and y may be the same rows (same type and stride); otherwise they must not overlap. */
+ * back).  layout: pairs are (i, i + rot_dim / 2) (half) or (2i, 2i + 1) (interleaved).  dim even, at most 2048.  Angles are within
+ * 2e-9 radians of pos * f_i at every position (f_i above 1: times f_i); sines, cosines and products are f32.  x and y may be
+ * the same rows (same type and stride); otherwise they must not overlap. */
 OJAS_B200_API int ojas_b200_rope_rows(ojas_b200_ctx *ctx, const ojas_b200_rope *rope, int layout, uint32_t x_type, const void *x, size_t x_stride,
                                       uint32_t y_type, void *y, size_t y_stride, const int32_t *pos, size_t M, size_t heads, size_t dim);
 OJAS_B200_API int ojas_b200_rope_rows_check(size_t rot_dim, int layout, uint32_t x_type, const void *x, size_t x_stride, uint32_t y_type,

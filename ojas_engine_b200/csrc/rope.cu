@@ -4,15 +4,21 @@
 // (x[2i], x[2i + 1]) (interleaved); elements from rot_dim on pass through.
 //
 // Angles: a 32-bit product pos * f_i is wrong by 0.06 radians at position 10^6.  The frequency is kept in turns as a 64-bit
-// binary fraction instead: pos * turns wraps modulo 2^64, i.e. modulo one turn, without any rounding, and its top bits go to
-// sincospi.  What is left is the rounding of f_i to 2^-64 turns and of the fraction to 32 bits (2^-32 turns = 1.5e-9 rad).
+// binary fraction instead: pos * turns wraps modulo 2^64, i.e. modulo one turn, without any rounding; rope_angle uses 56 bits of it.
+// What is left is the frequency's own error times the position, so it is formed with 64-bit significands: steps of 2^-64 of f_i in pow,
+// the scaling and the division by 2 pi, and half of 2^-64 turns, together below 2^-61 radians for f_i up to 1, 1e-9 radians at position
+// 2^31.  (From a double's 53 bits it was 2.6e-7.)
+#include <float.h>
 #include <math.h>
 
 #include "attn.cuh"
 #include "rope.cuh"
 
-// The frequencies in radians per position (host, 64 bits).
-static int rope_frequencies(size_t rot_dim, double base, const ojas_b200_rope_scaling *sc, const float *freq_factors, double *f, char *err, size_t errlen) {
+static_assert(LDBL_MANT_DIG >= 64, "frequencies are formed with 64-bit significands");
+constexpr long double TWO_PI = 6.283185307179586476925286766559005768L;
+
+// The frequencies in radians per position (host).
+static int rope_frequencies(size_t rot_dim, double base, const ojas_b200_rope_scaling *sc, const float *freq_factors, long double *f, char *err, size_t errlen) {
     auto no = [&](const char *why) { if (err && errlen) snprintf(err, errlen, "rope: %s", why); return OJAS_B200_E_ARG; };
     if (rot_dim < 2 || rot_dim % 2 != 0 || rot_dim > 1024) return no("rot_dim must be even, 2..1024");
     if (!(base > 1.0) || !isfinite(base)) return no("base must be a finite number above 1");
@@ -21,15 +27,15 @@ static int rope_frequencies(size_t rot_dim, double base, const ojas_b200_rope_sc
     if (sc && !(sc->magnitude > 0.0f && isfinite(sc->magnitude))) return no("magnitude must be positive");
     if (sc && sc->orig_len && !(fast > slow && slow >= 0.0 && isfinite(fast))) return no("beta_fast must be above beta_slow, both finite and not negative");
     for (size_t i = 0; i < rot_dim / 2; i++) {
-        f[i] = pow(base, -2.0 * (double)i / (double)rot_dim);
+        f[i] = powl((long double)base, -2.0L * (long double)i / (long double)rot_dim);
         if (freq_factors) {
             if (!(freq_factors[i] > 0.0f) || !isfinite(freq_factors[i])) return no("frequency factors must be positive");
-            f[i] /= (double)freq_factors[i];
+            f[i] /= (long double)freq_factors[i];
         }
         if (sc && sc->orig_len) {                 // by parts: pairs that turn often within the original context keep their frequency
-            double keep = ((double)sc->orig_len * f[i] / (2.0 * M_PI) - slow) / (fast - slow);
-            keep = keep < 0.0 ? 0.0 : keep > 1.0 ? 1.0 : keep;
-            f[i] = f[i] * keep + f[i] / factor * (1.0 - keep);
+            long double keep = ((long double)sc->orig_len * f[i] / TWO_PI - slow) / ((long double)fast - slow);
+            keep = keep < 0.0L ? 0.0L : keep > 1.0L ? 1.0L : keep;
+            f[i] = f[i] * keep + f[i] / factor * (1.0L - keep);
         } else {
             f[i] /= factor;
         }
@@ -40,20 +46,24 @@ static int rope_frequencies(size_t rot_dim, double base, const ojas_b200_rope_sc
 extern "C" int ojas_b200_rope_frequencies(size_t rot_dim, double base, const ojas_b200_rope_scaling *scaling, const float *freq_factors,
                                           double *radians_out, char *err, size_t errlen) {
     if (!radians_out) return OJAS_B200_E_ARG;
-    return rope_frequencies(rot_dim, base, scaling, freq_factors, radians_out, err, errlen);
+    long double f[512];
+    const int rc = rope_frequencies(rot_dim, base, scaling, freq_factors, f, err, errlen);
+    for (size_t i = 0; !rc && i < rot_dim / 2; i++) radians_out[i] = (double)f[i];
+    return rc;
 }
 
 extern "C" int ojas_b200_rope_create(ojas_b200_ctx *ctx, size_t rot_dim, double base, const ojas_b200_rope_scaling *scaling, const float *freq_factors,
                                      ojas_b200_rope **out) {
     if (!ctx || !out) return OJAS_B200_E_ARG;
     *out = nullptr;
-    double f[512];
+    long double f[512];
     uint64_t turns[512];
     const int rc = rope_frequencies(rot_dim, base, scaling, freq_factors, f, ctx->err, sizeof ctx->err);
     if (rc) return rc;
     for (size_t i = 0; i < rot_dim / 2; i++) {
-        const double t = f[i] / (2.0 * M_PI), frac = t - floor(t);           // below one turn per position in all real uses
-        turns[i] = (uint64_t)ldexp(frac, 64);                                // a double has 53 bits: exact
+        const long double t = f[i] / TWO_PI, frac = t - floorl(t);           // below one turn per position in all real uses
+        const long double steps = floorl(ldexpl(frac, 64) + 0.5L);
+        turns[i] = steps < 18446744073709551616.0L ? (uint64_t)steps : 0u;   // (rounded up to a whole turn)
     }
     DeviceGuard guard(ctx->device);
     uint64_t *dev = nullptr;

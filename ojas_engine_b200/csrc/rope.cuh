@@ -5,13 +5,15 @@
 #include "attn.cuh"
 
 // cos and sin of pos * turns[i] turns, times the magnitude.  The product modulo 2^64 read as a signed fraction is the angle in
-// (-1/2, 1/2] turns; the position may be negative (two's complement).
+// [-1/2, 1/2) turns; the position may be negative (two's complement).  An f32 holds the fraction's top 24 bits; the next 32, at most
+// 3.7e-7 radians, turn sine and cosine to first order (the second is below 1e-13).  (Rounded to an f32 alone, the angle is off by up to 9.4e-8.)
 __device__ __forceinline__ float2 rope_angle(int pos, uint64_t turns, float magnitude) {
-    const int64_t frac = (int64_t)((uint64_t)(int64_t)pos * turns);
-    const float half_turns = (float)(int)(frac >> 32) * 4.656612873077393e-10f;   // 2^-31: units of pi
+    const uint64_t frac = (uint64_t)(int64_t)pos * turns;
+    const int top = (int)(uint32_t)(frac >> 32) & ~0xff;
+    const float rest = (float)(uint32_t)(frac >> 8) * 8.7196693e-17f;             // pi 2^-55: radians
     float s, c;
-    sincospif(half_turns, &s, &c);
-    return make_float2(c * magnitude, s * magnitude);
+    sincospif((float)top * 4.656612873077393e-10f, &s, &c);                       // 2^-31: units of pi
+    return make_float2(fmaf(-s, rest, c) * magnitude, fmaf(c, rest, s) * magnitude);
 }
 
 // Units a head is cut into: VEC pairs each, then 2 VEC passing elements each.

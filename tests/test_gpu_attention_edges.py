@@ -1,4 +1,7 @@
 """Descriptions, lengths and shapes at the edge of what append and attention take, on the GPU; beside test_gpu_attention.py."""
+import decimal
+import math
+
 import pytest
 import torch
 
@@ -13,6 +16,42 @@ HALVES, INTER = ob.ROPE_HALF, ob.ROPE_INTERLEAVED
 
 def randn(seed, *shape, dtype=torch.float32):
     return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).to(dtype)
+
+
+# -------------------------------------------------------------------------------------------------------------- rotation
+PI = decimal.Decimal("3.14159265358979323846264338327950288419716939937510582097494459230781640628620899")
+
+
+def turns_128(rot, base):
+    """Turns per position of each pair, base^(-2i / rot) / 2 pi, as integers over 2^128, formed in 60 digits."""
+    with decimal.localcontext(prec=60):
+        ln = decimal.Decimal(base).ln()
+        return [int((-2 * i * ln / rot).exp() / (2 * PI) * 2**128) for i in range(rot // 2)]
+
+
+@pytest.mark.parametrize("base", [10000, 500000])
+@pytest.mark.parametrize("near", [0, 131072, 2**24 + 1, -(10**9), 2**31 - 2001, -(2**31)])
+def test_angles_at_every_position(gpu, base, near):
+    """Angles within 2e-9 radians: seen where a sine or a cosine is below 2^-8, whose own rounding (sincospi, one correction, one
+    product: four steps of 2^-23 relative at most) then stays below 2e-9 too."""
+    rot, n = 128, 2001
+    pos = torch.arange(near, near + n, dtype=torch.int64)
+    x = torch.zeros(n, 1, rot)
+    x[..., : rot // 2] = 1.0
+    xd, pd, rope = x.cuda(), pos.to(torch.int32).cuda(), ob.Rope(gpu, rot, base=float(base))
+    torch.cuda.synchronize()
+    gpu.rope_rows(rope, buf(xd), buf(xd), buf(pd), n, 1, rot)
+    gpu.sync()
+    got = xd.cpu().double()[:, 0]
+    turns, whole = turns_128(rot, base), 2**128
+    frac = torch.tensor([[((p * t + whole // 2) % whole - whole // 2) / whole for t in turns] for p in pos.tolist()], dtype=torch.float64)
+    worst = 0.0
+    for value, want in ((got[:, : rot // 2], torch.cos(2 * math.pi * frac)), (got[:, rot // 2 :], torch.sin(2 * math.pi * frac))):
+        small = want.abs() < 2.0**-8
+        assert near == 0 or small.sum() > 100
+        worst = max(worst, ((value - want).abs() - 4 * 2.0**-23 * want.abs())[small].max().item())
+        assert ((value - want).abs() <= 2e-9 + 4 * 2.0**-23).all()
+    assert worst <= 2e-9, worst
 
 
 # ---------------------------------------------------------------------------------------------------------------- append
