@@ -39,6 +39,7 @@ static int rope_frequencies(size_t rot_dim, double base, const ojas_b200_rope_sc
         } else {
             f[i] /= factor;
         }
+        if (!isfinite((double)f[i])) return no("a frequency is not finite");
     }
     return 0;
 }
