@@ -82,6 +82,11 @@ class B200Gpu:
 
     def close(self) -> None:
         if getattr(self, "_ctx", None):
+            if self._attn_ws:
+                self._l.ojas_b200_sync(self._ctx)             # (whatever it reports: the work has ended)
+                for buf in self._attn_ws:
+                    self._l.ojas_b200_free(self._ctx, C.c_void_p(buf.ptr))
+                self._attn_ws.clear()
             self._l.ojas_b200_destroy(self._ctx)
             self._ctx = None
 
@@ -300,8 +305,8 @@ class B200Gpu:
     def attention(self, kv: KvCache, seqs: Seqs, q: Buf, out: Buf, m: int, q_heads: int, act_type: int = F32, scale: float | None = None,
                   causal: bool = True, window: int = 0, q_stride: int = 0, out_stride: int = 0, workspace: Buf | None = None) -> None:
         """Attention of the call's rows over their sequences' keys (scale: 1 / sqrt(dim) unless given).  Without a caller
-        workspace a grow-only scratch buffer owned by this object is used; a buffer it outgrew stays allocated, because a
-        captured graph may still use it.  It grows by an allocation: make a shape's first call outside a capture."""
+        workspace a grow-only scratch buffer owned by this object is used; a buffer it outgrew stays allocated until ``close``,
+        because a captured graph may still use it.  It grows by an allocation: make a shape's first call outside a capture."""
         if workspace is None:
             shape = (kv.heads, kv.dim, kv.page_size, kv.type, act_type, m, q_heads, window, self._ctx.value)
             need = seqs._need.get(shape)

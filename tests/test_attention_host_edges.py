@@ -3,6 +3,7 @@ import numpy as np
 import pytest
 
 import ojas_engine_b200 as ob
+from ojas_engine_b200 import runtime
 
 
 @pytest.mark.parametrize("kw", [dict(factor=5e-324), dict(factor=1e-308, freq_factors=[1e-3] * 32)])
@@ -16,3 +17,90 @@ def test_a_factor_that_no_pair_is_divided_by():
     far the divided one would lie beyond a double."""
     got = ob.rope_frequencies(64, factor=1e-308, freq_factors=[1e-3] * 32, orig_len=4096)
     assert np.allclose(got, ob.rope_frequencies(64, freq_factors=[1e-3] * 32), rtol=1e-15, atol=0)
+
+
+class FakeLibrary:
+    """The calls a B200Gpu makes of the library around attention, recorded; device memory is numbers."""
+
+    def __init__(self, workspace=4096, context=0x1000):
+        self.calls, self.live, self.workspace, self.context, self.next = [], {}, workspace, context, 0x100000
+
+    def ojas_b200_create(self, device, stream, out):
+        out._obj.value = self.context
+        return 0
+
+    def ojas_b200_destroy(self, ctx):
+        self.calls.append("destroy")
+
+    def ojas_b200_sync(self, ctx):
+        self.calls.append("sync")
+        return 0
+
+    def ojas_b200_alloc(self, ctx, nbytes, out):
+        self.next += 0x10000
+        self.live[self.next] = nbytes
+        out._obj.value = self.next
+        return 0
+
+    def ojas_b200_free(self, ctx, ptr):
+        self.calls.append("free")
+        del self.live[ptr.value]
+        return 0
+
+    def ojas_b200_last_error(self, ctx):
+        return b""
+
+    def ojas_b200_kv_create(self, *args):
+        args[-1]._obj.value = 0x2000
+        return 0
+
+    def ojas_b200_kv_destroy(self, h):
+        pass
+
+    def ojas_b200_attention_workspace_bytes(self, *args):
+        return self.workspace
+
+    def ojas_b200_attention(self, *args):
+        self.calls.append(("attention", args[-1]))
+        return 0
+
+
+def fake_gpu(monkeypatch, **kw):
+    fake = FakeLibrary(**kw)
+    monkeypatch.setattr(runtime._lib, "load", lambda: fake)
+    return fake, ob.B200Gpu(0)
+
+
+def fake_call(gpu, seqs=None, m=1):
+    kv = ob.KvCache(gpu, ob.F16, ob.Buf(4096, 1 << 30), ob.Buf(4096, 1 << 30), 4, 16, 2, 128)
+    seqs = seqs or ob.Seqs(ob.Buf(0, 8), ob.Buf(0, 4), ob.Buf(0, 16), 1, 4, m, 60)
+    gpu.attention(kv, seqs, ob.Buf(0, 1 << 20), ob.Buf(0, 1 << 20), m, 4)
+    return seqs
+
+
+def test_closing_frees_the_scratch(monkeypatch):
+    """Scratch a context grew through belongs to it: freed once its work has ended, before the context itself."""
+    fake, gpu = fake_gpu(monkeypatch)
+    fake_call(gpu)
+    fake.workspace = 100000
+    fake_call(gpu, m=2)
+    assert len(fake.live) == 2                                 # a captured graph may use the first
+    gpu.close()
+    assert not fake.live
+    assert fake.calls[-4:] == ["sync", "free", "free", "destroy"]
+    gpu.close()                                                # twice: nothing more
+    assert fake.calls.count("destroy") == 1
+
+
+def test_closing_an_unused_context_does_not_wait(monkeypatch):
+    fake, gpu = fake_gpu(monkeypatch)
+    gpu.close()
+    assert fake.calls == ["destroy"]
+
+
+def test_closing_after_an_error_still_frees(monkeypatch):
+    fake, gpu = fake_gpu(monkeypatch)
+    fake_call(gpu)
+    fake.ojas_b200_sync = lambda ctx: -5
+    gpu.close()
+    assert not fake.live and fake.calls[-1] == "destroy"
