@@ -11,6 +11,7 @@ computes through the C ABI; nothing here falls back to the CPU.
 from __future__ import annotations
 
 import ctypes as C
+import itertools
 from dataclasses import dataclass
 
 import numpy as np
@@ -63,6 +64,9 @@ class Enc:
         self.dispatches = 0
 
 
+_serials = itertools.count()
+
+
 class B200Gpu:
     def __init__(self, device: int = 0, stream: int | None = None):
         self._l = _lib.load()
@@ -74,6 +78,7 @@ class B200Gpu:
         self._ctx = ctx
         self.device = device
         self._attn_ws: list[Buf] = []
+        self._serial = next(_serials)              # no other context has it, not even a later one at the same address
 
     # ------------------------------------------------------------------ plumbing
     def _ck(self, rc: int) -> None:
@@ -308,7 +313,7 @@ class B200Gpu:
         workspace a grow-only scratch buffer owned by this object is used; a buffer it outgrew stays allocated until ``close``,
         because a captured graph may still use it.  It grows by an allocation: make a shape's first call outside a capture."""
         if workspace is None:
-            shape = (kv.heads, kv.dim, kv.page_size, kv.type, act_type, m, q_heads, window, self._ctx.value)
+            shape = (kv.heads, kv.dim, kv.page_size, kv.type, act_type, m, q_heads, window, self._serial)
             need = seqs._need.get(shape)
             if need is None:                       # depends on the bounds and counts alone, which a Seqs does not change
                 need = seqs._need[shape] = self.attention_workspace_bytes(kv, seqs, m, q_heads, act_type, window)

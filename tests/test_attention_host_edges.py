@@ -104,3 +104,24 @@ def test_closing_after_an_error_still_frees(monkeypatch):
     fake.ojas_b200_sync = lambda ctx: -5
     gpu.close()
     assert not fake.live and fake.calls[-1] == "destroy"
+
+
+def test_the_workspace_is_asked_for_by_the_context_in_use(monkeypatch):
+    """A Seqs outlives its context and a new one gets the old one's address: what the old one needed says nothing about the new one."""
+    fake, gpu = fake_gpu(monkeypatch)
+    seqs = fake_call(gpu)
+    gpu.close()
+    fake, gpu = fake_gpu(monkeypatch, workspace=1 << 20)
+    fake_call(gpu, seqs)
+    assert fake.calls[-1] == ("attention", 1 << 20)
+
+
+def test_the_workspace_is_asked_for_once_per_shape(monkeypatch):
+    fake, gpu = fake_gpu(monkeypatch)
+    asked = []
+    fake.ojas_b200_attention_workspace_bytes = lambda *args: asked.append(args) or 4096
+    seqs = fake_call(gpu)
+    fake_call(gpu, seqs)
+    assert len(asked) == 1
+    fake_call(gpu, seqs, m=2)
+    assert len(asked) == 2
