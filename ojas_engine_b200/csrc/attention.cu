@@ -26,7 +26,7 @@
 constexpr int AR_KEYS = 64;                                  // keys of a block
 constexpr int AR_WARPS = 4, AR_THREADS = (AR_WARPS + 1) * 32;   // consumer warps; and the producer
 constexpr int AR_STAT_BYTES = 256 + AR_WARPS * 32 * 8 + 32 * 8;   // barriers; per warp and row (maximum, sum); per row the same
-constexpr int AR_CLUSTER = 16;                               // most splits that can be a cluster (more than 8 have to be asked for)
+constexpr int AR_CLUSTER = 16;                               // most splits that are a cluster (more than 8 have to be asked for; see cluster_limit)
 __host__ __device__ constexpr int ar_stage_bytes(int dim) { return 2 * AR_KEYS * dim * 2; }
 // 96 KB of blocks in flight per CTA, two CTAs per SM (dim 256: three 64 KB blocks, one CTA): HBM needs about 44 KB per SM and
 // microsecond of latency.
@@ -461,8 +461,41 @@ static int attn_shape_check(uint32_t cache_type, size_t page_size, size_t kv_hea
     return 0;
 }
 
+// The most splits of the kernel for few rows that the device can place as one cluster: up to 16 where two CTAs share an SM, up to 8 where
+// one has it (sixteen would need most of a GPC at once); fewer, or none (1), where its GPCs have fewer free SMs, as a partitioned device may.  Asked
+// once per device, of the instance that needs most.
+template <int D>
+static int placeable(int device, int most) {
+    static std::atomic<uint64_t> ready{0};
+    int fit = 0;
+    while (most > 1) {
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = (unsigned)most;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(1, 1, (unsigned)most); cfg.blockDim = dim3(AR_THREADS); cfg.dynamicSmemBytes = ar_smem(D);
+        cfg.attrs = attr; cfg.numAttrs = 1;
+        if (smem_once(ready, device, attn_rows_kernel<D, false, true, 1>, ar_smem(D), most > 8) == cudaSuccess &&
+            cudaOccupancyMaxActiveClusters(&fit, attn_rows_kernel<D, false, true, 1>, &cfg) == cudaSuccess && fit > 0) break;
+        cudaGetLastError();                                  // a refusal is an answer
+        most /= 2;
+    }
+    return most;
+}
+static int cluster_limit(int device, bool pairs) {
+    static std::atomic<int> known[2][32];                    // 0: not asked yet
+    int limit = device < 32 ? known[pairs][device].load(std::memory_order_relaxed) : 0;
+    if (limit == 0) {
+        DeviceGuard guard(device);
+        limit = pairs ? placeable<128>(device, AR_CLUSTER) : placeable<256>(device, AR_CLUSTER / 2);
+        if (device < 32) known[pairs][device].store(limit, std::memory_order_relaxed);
+    }
+    return limit;
+}
+
 // Which kernel, and how far the keys are split so that few rows still use every SM.
-static AttnPlan attn_plan(int sm_count, size_t n_seqs, size_t M, size_t max_rows, size_t max_len, size_t q_heads, size_t kv_heads, size_t dim, size_t window, bool f32) {
+static AttnPlan attn_plan(const ojas_b200_ctx *ctx, size_t n_seqs, size_t M, size_t max_rows, size_t max_len, size_t q_heads, size_t kv_heads, size_t dim, size_t window, bool f32) {
     AttnPlan p{};
     const size_t group = q_heads / kv_heads, bound = (max_rows < M ? max_rows : M) * group;
     p.two = f32 || bound <= 8;
@@ -487,9 +520,9 @@ static AttnPlan attn_plan(int sm_count, size_t n_seqs, size_t M, size_t max_rows
     // cost a launch, and the bytes of their sums.  (One 131 000-key pair of sequences: 135 us in 16 to 18 splits, 150 in 63; 64 ragged sequences of up to 8192
     // keys: 202 us in one split, 186 in 3 or 4, 214 in 12; 16 of up to 6000 with dim 256: 132, 43 in 4, 37 in 6, 50 in 16.)
     const bool pairs = dim != 256 && p.mt == 1 && !p.tensor;
-    const double slots = (double)sm_count * (pairs ? 2 : 1), fixed = pairs ? 3.0 : 6.0, part = 0.5 + 0.5 / (double)n_seqs;
+    const double slots = (double)ctx->sm_count * (pairs ? 2 : 1), fixed = pairs ? 3.0 : 6.0, part = 0.5 + 0.5 / (double)n_seqs;
     const double sums = 0.25 + (double)M * (double)q_heads * (double)dim * 4.0 / 6.75e6;
-    const int largest = pairs ? AR_CLUSTER : AR_CLUSTER / 2; // with one CTA per SM sixteen would need most of a GPC at once
+    const int largest = p.tensor ? 1 : cluster_limit(ctx->device, pairs);
     double best = 0.0;
     int splits = 1;
     for (int n = 1; n <= 64 && n * 2 <= (int)blocks; n = n < 8 ? n + 1 : n + n / 4) {
@@ -531,7 +564,7 @@ extern "C" size_t ojas_b200_attention_workspace_bytes(ojas_b200_ctx *ctx, const 
                                                       long long window) {
     if (!ctx || !kv || !seqs || window < 0 || M == 0 || seqs->n_seqs == 0) return 0;
     if (attn_shape_check(kv->type, kv->page_size, kv->heads, kv->dim, act_type, q_heads, M, seqs->max_rows, seqs->max_len, nullptr, 0)) return 0;
-    return attn_plan(ctx->sm_count, seqs->n_seqs, M, seqs->max_rows, seqs->max_len, q_heads, kv->heads, kv->dim, (size_t)window, act_type == OJAS_B200_F32).workspace;
+    return attn_plan(ctx, seqs->n_seqs, M, seqs->max_rows, seqs->max_len, q_heads, kv->heads, kv->dim, (size_t)window, act_type == OJAS_B200_F32).workspace;
 }
 
 template <int D, bool BF, bool TWO, int MT>
@@ -579,7 +612,7 @@ extern "C" int ojas_b200_attention(ojas_b200_ctx *ctx, const ojas_b200_kv *kv, c
     const int rc = ojas_b200_attention_check(kv->type, kv->page_size, kv->heads, kv->dim, act_type, q_heads, q, q_stride, out, out_stride, scale, causal, window, seqs, M, why, sizeof why);
     if (rc) return ojas_fail(ctx, rc, "%s", why);
     if (M == 0 || seqs->n_seqs == 0) return 0;
-    const AttnPlan p = attn_plan(ctx->sm_count, seqs->n_seqs, M, seqs->max_rows, seqs->max_len, q_heads, kv->heads, kv->dim, (size_t)window, act_type == OJAS_B200_F32);
+    const AttnPlan p = attn_plan(ctx, seqs->n_seqs, M, seqs->max_rows, seqs->max_len, q_heads, kv->heads, kv->dim, (size_t)window, act_type == OJAS_B200_F32);
     if (p.workspace) {
         if (!workspace || workspace_bytes < p.workspace) return ojas_fail(ctx, OJAS_B200_E_ARG, "attention: workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : 0, p.workspace);
         if ((uintptr_t)workspace % 256) return ojas_fail(ctx, OJAS_B200_E_ARG, "attention: the workspace must start on 256 bytes");

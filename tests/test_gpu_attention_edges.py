@@ -151,3 +151,18 @@ def test_a_wrong_batch_and_a_lost_wait_are_both_named(gpu):
         assert ("batch" in str(e.value)) == batch and ("bounded wait" in str(e.value)) == wait
     group.close()
     gpu.free(y)
+
+
+@pytest.mark.parametrize("dim,q_heads", [(64, 8), (128, 32), (256, 16)])
+def test_one_short_sequence_joins_in_one_launch(gpu, dim, q_heads):
+    """A B200 places the clusters that the splits of a short sequence make: no workspace, no second launch."""
+    b = Batch([1], [900], kv_heads=q_heads // 4, dim=dim, seed=3).upload(gpu)
+    assert gpu.attention_workspace_bytes(b.kv, b.seqs, 1, q_heads) == 0
+    q = randn(1, 1, q_heads, dim)
+    qd, out, before = q.cuda(), torch.empty(1, q_heads, dim).cuda(), gpu.launch_count
+    torch.cuda.synchronize()
+    gpu.attention(b.kv, b.seqs, buf(qd), buf(out), 1, q_heads)
+    gpu.sync()
+    assert gpu.launch_count == before + 1
+    want, weight, vmax = b.attention_exact(q, q_heads)
+    check(out, want, attention_bound(want, weight, vmax, dim, 900, F32, F16, 2))
