@@ -166,3 +166,155 @@ def test_one_short_sequence_joins_in_one_launch(gpu, dim, q_heads):
     assert gpu.launch_count == before + 1
     want, weight, vmax = b.attention_exact(q, q_heads)
     check(out, want, attention_bound(want, weight, vmax, dim, 900, F32, F16, 2))
+
+
+# ------------------------------------------------------------------------------------------------------- long loops, splits
+def exact_on_gpu(b, q, hq, causal=True, window=0):
+    """Batch.attention_exact by the GPU's 64-bit units, for sizes that take the host too long: out and the scores' sizes."""
+    d, group = b.dim, hq // b.hk
+    out, weight = (torch.zeros(b.M, hq, n, dtype=torch.float64) for n in (d, 1))
+    for i, (n, total) in enumerate(zip(b.rows, b.lens)):
+        t0, key = int(b.cu[i]), torch.arange(total).cuda()
+        pos = torch.arange(total - n, total).cuda()[:, None]
+        seen = (key <= pos) & (key > pos - (window or total)) if causal else (key >= 0).expand(n, total)
+        for h in range(b.hk):
+            k, v = b.k_rows[i][:, h].cuda().double(), b.v_rows[i][:, h].cuda().double()
+            for j in range(h * group, (h + 1) * group):
+                x = q[t0 : t0 + n, j].cuda().double()
+                s = (x @ k.T * d**-0.5).masked_fill_(~seen, -math.inf)
+                out[t0 : t0 + n, j] = (torch.softmax(s, -1) @ v).cpu()
+                weight[t0 : t0 + n, j] = (x.abs() @ k.abs().T * d**-0.5).masked_fill_(~seen, 0.0).amax(-1, keepdim=True).cpu()
+    return out, weight
+
+
+def attend(gpu, b, q, hq, act, window=0, causal=True):
+    qd = q.to(TORCH[act]).cuda()
+    out = torch.full_like(qd, 77.0)
+    torch.cuda.synchronize()
+    gpu.attention(b.kv, b.seqs, buf(qd), buf(out), b.M, hq, act_type=act, window=window, causal=causal)
+    gpu.sync()
+    return out
+
+
+def splits(gpu, b, hq, act, window=0):
+    """In how many parts the keys of a call that joins through its workspace are split (1: it needs none)."""
+    need = gpu.attention_workspace_bytes(b.kv, b.seqs, b.M, hq, act, window)
+    return max(1, need // (b.M * hq * (8 + 4 * b.dim)))
+
+
+FLUSH = 512                                                    # keys after which f32 results are added to rounded sums
+
+
+@pytest.mark.parametrize("dim,tokens,heads,split", [(64, 200, 8, False), (128, 200, 8, False), (256, 200, 8, True), (256, 288, 8, False), (64, 160, 4, True),
+                                                    (128, 160, 4, True), (256, 160, 4, True), (64, 30, 1, True), (128, 30, 1, True), (256, 30, 1, True)])
+def test_sums_of_many_keys_keep_f32_precision(gpu, dim, tokens, heads, split):
+    """f32 activations, 12 000 keys of nearly equal weight, values between 1 and 2: everything the accumulator loses has one sign.
+    Between two roundings into the sums it takes 512 keys: 2 * 512 / 16 instructions that cut up to 2^-23 of what has grown so far, half of
+    the whole on average, so 32 steps of 2^-23; then one rounded addition per 512 keys and per split; the rest as in attention_bound, with
+    scores small enough not to matter.  (Without the sums: 1500 instructions, 750 steps at most, 280 on average.)"""
+    group, keys = 8, 12000
+    b = Batch([tokens], [keys], kv_heads=heads, dim=dim, page=64, seed=dim)
+    b.v_rows[0] = (1 + torch.rand(keys, heads, dim, generator=b.g)).half()
+    b.put(b.v, 0, 0, b.v_rows[0])
+    b.upload(gpu)
+    n = splits(gpu, b, heads * group, F32)
+    assert (n > 1) == split and (tokens == 30 or keys / n > 3 * FLUSH + 128)         # three flushes at least in one CTA
+    q = randn(1, tokens, heads * group, dim) * 0.01
+    want, weight = exact_on_gpu(b, q, heads * group)
+    steps = 32 + keys / FLUSH + n + 16
+    rel = 2 * (weight * ((dim / 16 + 4) * 2.0**-23 + 2 * 2.0**-22 + 2.0**-22) + 2.0**-21) + 2 * 2.0**-22 + steps * 2.0**-23
+    check(attend(gpu, b, q, heads * group, F32), want, 2 * rel + 2.0**-24 * want)
+
+
+@pytest.mark.parametrize("act,cache", [(F32, F16), (F32, BF16), (F16, F16), (BF16, BF16)])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("tokens,heads", [(200, 8), (160, 2)])
+def test_a_maximum_that_grows_along_the_keys(gpu, act, cache, dim, tokens, heads):
+    """Keys that grow all along a sequence of 4000: maxima rise in most blocks, before and after results were added to the sums."""
+    group, keys = 8, 4000
+    b = Batch([tokens], [keys], kv_heads=heads, dim=dim, page=32, cache=cache, seed=dim + tokens)
+    b.k_rows[0] = (b.k_rows[0].float() * torch.linspace(0.02, 3, keys)[:, None, None]).to(TORCH[cache])
+    b.put(b.k, 0, 0, b.k_rows[0])
+    b.upload(gpu)
+    q = randn(1, tokens, heads * group, dim).to(TORCH[act])
+    want, weight = exact_on_gpu(b, q, heads * group)
+    vmax = b.v_rows[0].double().abs().max()
+    check(attend(gpu, b, q, heads * group, act), want, attention_bound(want, weight, vmax, dim, keys, act, cache, 2 if act == F32 else 1))
+
+
+@pytest.mark.parametrize("act,cache", [(F32, F16), (F32, BF16), (F16, F16), (BF16, BF16)])
+@pytest.mark.parametrize("dim,rows,lens,heads,group,window", [
+    (64, [2500], [2500], 8, 4, 0), (128, [2200], [3001], 4, 4, 0), (256, [1500], [2000], 4, 4, 0),               # prompts, keys not split
+    (64, [900, 1, 70], [3300, 2047, 1000], 2, 7, 0), (128, [300, 5], [4100, 4000], 1, 8, 0), (256, [40, 200], [5000, 999], 2, 2, 0),
+    (64, [3000], [3000], 4, 2, 500), (128, [1000, 1000], [1000, 2500], 4, 4, 777), (256, [700], [1700], 2, 4, 64),
+    (64, [1, 1, 1], [6000, 1, 2049], 2, 8, 0), (128, [1, 3], [9000, 500], 1, 4, 0), (256, [1, 2], [7000, 65], 2, 4, 0), (128, [4], [5000], 2, 3, 1000)])
+def test_every_key_counts_once(gpu, act, cache, dim, rows, lens, heads, group, window):
+    """Value j is the unit vector of j modulo dim: an element of the result is the weight of every dim-th key, and is off by a
+    relative error only.  One key too many or too few among the some tens of an element is beyond any rounding."""
+    b = Batch(rows, lens, kv_heads=heads, dim=dim, page=16, cache=cache, seed=dim + len(rows))
+    for i, n in enumerate(lens):
+        b.v_rows[i] = torch.eye(dim).repeat((n + dim - 1) // dim, 1)[:n, None].expand(n, heads, dim).to(TORCH[cache]).contiguous()
+        b.put(b.v, i, 0, b.v_rows[i])
+    b.upload(gpu)
+    q = (randn(1, b.M, heads * group, dim) * 0.3).to(TORCH[act])
+    want, weight = exact_on_gpu(b, q, heads * group, window=window)
+    bound = attention_bound(want, weight, want, dim, max(lens), act, cache, 2 if act == F32 else 1)
+    check(attend(gpu, b, q, heads * group, act, window=window), want, bound)
+
+
+@pytest.mark.parametrize("act,cache", [(F32, F16), (BF16, BF16)])
+@pytest.mark.parametrize("dim,rows,group", [(64, [1, 3, 1], 4), (64, [2, 1, 1], 14), (128, [1, 1, 2], 8), (256, [1, 2, 1], 4), (256, [3, 1, 1], 5)])
+def test_few_rows_joined_through_the_workspace(gpu, act, cache, dim, rows, group):
+    """More splits than a cluster has, planned for lengths far beyond the actual ones: long, short and single-block sequences."""
+    b = Batch(rows, [6000, 700, 9], kv_heads=1, dim=dim, cache=cache, seed=dim, max_len=500000).upload(gpu)
+    assert splits(gpu, b, group, act) > 16
+    q = randn(2, b.M, group, dim).to(TORCH[act])
+    want, weight, vmax = b.attention_exact(q, group)
+    check(attend(gpu, b, q, group, act), want, attention_bound(want, weight, vmax, dim, 6000, act, cache, 2 if act == F32 else 1))
+
+
+@pytest.mark.parametrize("rows,max_len", [(1, 500000), (60, 9000)])
+def test_two_streams_with_a_workspace_each(gpu, rows, max_len):
+    """Two contexts on streams of their own, splits that join through scratch, different queries: neither sees the other's."""
+    b = Batch([rows, rows], [9000, 4000], kv_heads=2, dim=128, seed=5, max_len=max_len).upload(gpu)
+    qs = [randn(seed, b.M, 8, 128) for seed in (3, 4)]
+    exact = [b.attention_exact(q, 8) for q in qs]
+    others, on_gpu = [ob.B200Gpu(0) for _ in qs], [q.cuda() for q in qs]
+    outs = [torch.empty(b.M, 8, 128).cuda() for _ in qs]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for o, q, out in zip(others, on_gpu, outs):
+            assert o.attention_workspace_bytes(b.kv, b.seqs, b.M, 8) > 0
+            o.attention(b.kv, b.seqs, buf(q), buf(out), b.M, 8)
+    for o, out, (want, weight, vmax) in zip(others, outs, exact):
+        o.sync()
+        check(out, want, attention_bound(want, weight, vmax, 128, 9000, F32, F16, 2))
+        o.close()
+
+
+@pytest.mark.parametrize("rows,max_len", [(1, 500000), (60, 9000)])
+def test_two_graphs_share_a_workspace_in_turn(gpu, rows, max_len):
+    b = Batch([rows, rows], [5000, 300], kv_heads=2, dim=128, seed=5, max_len=max_len).upload(gpu)
+    assert gpu.attention_workspace_bytes(b.kv, b.seqs, b.M, 8) > 0
+    qs = [randn(seed, b.M, 8, 128) for seed in (3, 4)]
+    on_gpu, outs = [q.cuda() for q in qs], [torch.empty(b.M, 8, 128).cuda() for _ in qs]
+    torch.cuda.synchronize()
+    gpu.attention(b.kv, b.seqs, buf(on_gpu[0]), buf(outs[0]), b.M, 8)
+    gpu.sync()
+    graphs = []
+    for q, out in zip(on_gpu, outs):
+        gpu.graph_begin()
+        gpu.attention(b.kv, b.seqs, buf(q), buf(out), b.M, 8)
+        graphs.append(gpu.graph_end())
+    first = None
+    for _ in range(5):
+        for gr in graphs:
+            gpu.graph_launch(gr)
+        gpu.sync()
+        first = first or [o.clone() for o in outs]
+        assert all(torch.equal(a, o) for a, o in zip(first, outs))
+    for q, out in zip(qs, outs):
+        want, weight, vmax = b.attention_exact(q, 8)
+        check(out, want, attention_bound(want, weight, vmax, 128, 5000, F32, F16, 2))
+    for gr in graphs:
+        gpu.graph_destroy(gr)
