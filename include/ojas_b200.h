@@ -356,7 +356,7 @@ OJAS_B200_API int ojas_b200_kv_append_check(size_t kv_heads, size_t dim, size_t 
 /* out[row, h] = softmax_j(scale * q[row, h] . k_j) v_j over the keys the row sees: of its sequence's first len[b] keys those
  * up to its own position (causal != 0), or all of them; with window > 0 (causal only) at most the last `window`, its own
  * included.  q head h reads cache head h / (q_heads / heads).  A row that sees nothing gives zeros.  q and out have type
- * act_type: f32, or the cache's type; they start on 16 bytes, strides are multiples of 4 elements, and they must not overlap.
+ * act_type: f32, or the cache's type; scale * log2(e) is finite in f32; they start on 16 bytes, strides are multiples of 4 elements, and they must not overlap.
  * f32 activations keep 22 bits through both products over an f16 cache, 16 over a bf16 cache; 16-bit ones are rounded where
  * the probabilities enter the second product and at the end.  Sums and softmax statistics are f32.
  * Behind a sequence's end the cache may hold anything; a key that only some rows of a call see must be finite for the

@@ -448,6 +448,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a) {
 }
 
 // ---------------------------------------------------------------------------- plan
+constexpr float LOG2_E = 1.4426950408889634f;
 static int attn_shape_check(uint32_t cache_type, size_t page_size, size_t kv_heads, size_t dim, uint32_t act_type, size_t q_heads, size_t M, size_t max_rows,
                             size_t max_len, char *err, size_t errlen) {
     auto no = [&](int code, const char *why) { if (err && errlen) snprintf(err, errlen, "attention: %s", why); return code; };
@@ -547,7 +548,7 @@ extern "C" int ojas_b200_attention_check(uint32_t cache_type, size_t page_size, 
     if (rc) return rc;
     rc = attn_shape_check(cache_type, page_size, kv_heads, dim, act_type, q_heads, M, seqs->max_rows, seqs->max_len, err, errlen);
     if (rc) return rc;
-    if (!(scale == scale) || scale - scale != 0.0f) return no(OJAS_B200_E_ARG, "the scale must be finite");
+    if (!isfinite(scale * LOG2_E)) return no(OJAS_B200_E_ARG, "the scale, in powers of two, must be finite");
     if (window < 0 || window > 0x7fffffff) return no(OJAS_B200_E_ARG, "the window must be 0 (none) or a number of keys");
     if (window && !causal) return no(OJAS_B200_E_UNSUPPORTED, "a window needs causal rows");
     if ((q_stride && q_stride < q_heads * dim) || (out_stride && out_stride < q_heads * dim)) return no(OJAS_B200_E_ARG, "a row stride is smaller than a row");
@@ -626,7 +627,7 @@ extern "C" int ojas_b200_attention(ojas_b200_ctx *ctx, const ojas_b200_kv *kv, c
     a.act_type = act_type; a.q_heads = (int)q_heads; a.group = (int)(q_heads / kv->heads);
     a.splits = p.splits; a.split_blocks = p.split_blocks; a.per_seq = p.per_seq;
     a.window = (int)window; a.causal = causal != 0;
-    a.scale_log2 = scale * 1.4426950408889634f;
+    a.scale_log2 = scale * LOG2_E;
     if (p.workspace) {
         a.part_ml = static_cast<float2 *>(workspace);
         a.part_o = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + align256((size_t)p.splits * M * q_heads * sizeof(float2)));

@@ -1,4 +1,6 @@
 """Host side of rotary positions, the paged cache and attention at its edges (no GPU); beside test_attention_host.py."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
@@ -125,3 +127,11 @@ def test_the_workspace_is_asked_for_once_per_shape(monkeypatch):
     assert len(asked) == 1
     fake_call(gpu, seqs, m=2)
     assert len(asked) == 2
+
+
+@pytest.mark.parametrize("scale,ok", [(0.0, True), (-0.5, True), (2.3e38, True), (2.4e38, False), (-3e38, False)])
+def test_a_scale_stays_finite_in_powers_of_two(scale, ok):
+    """Scores are formed in powers of two: the scale times log2(e) has to be a number, or equal scores of 0 were not."""
+    seqs = runtime._lib.SeqsStruct(256, 512, 1024, 3, 8, 4, 100)
+    rc = runtime._lib.load().ojas_b200_attention_check(ob.F16, 16, 2, 128, ob.F32, 8, 1024, 0, 4096, 0, scale, 1, 0, C.byref(seqs), 12, None, 0)
+    assert rc == (0 if ok else -1)

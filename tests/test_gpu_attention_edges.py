@@ -318,3 +318,17 @@ def test_two_graphs_share_a_workspace_in_turn(gpu, rows, max_len):
         check(out, want, attention_bound(want, weight, vmax, 128, 5000, F32, F16, 2))
     for gr in graphs:
         gpu.graph_destroy(gr)
+
+
+@pytest.mark.parametrize("act,cache", [(F32, F16), (F16, F16), (BF16, BF16)])
+@pytest.mark.parametrize("dim,rows", [(128, 1), (64, 5), (256, 2), (128, 60), (64, 300), (256, 100)])
+@pytest.mark.parametrize("scale", [0.0, -0.11, 1.5])
+def test_scales_of_any_sign(gpu, act, cache, dim, rows, scale):
+    b = Batch([rows, 1], [rows + 130, 77], kv_heads=2, dim=dim, cache=cache, seed=dim + rows).upload(gpu)
+    q = randn(1, b.M, 8, dim).to(TORCH[act])
+    qd, out = q.cuda(), torch.empty(b.M, 8, dim, dtype=TORCH[act]).cuda()
+    torch.cuda.synchronize()
+    gpu.attention(b.kv, b.seqs, buf(qd), buf(out), b.M, 8, act_type=act, scale=scale)
+    gpu.sync()
+    want, weight, vmax = b.attention_exact(q, 8, scale=scale)
+    check(out, want, attention_bound(want, weight, vmax, dim, max(b.lens), act, cache, 2 if act == F32 else 1))
