@@ -457,7 +457,7 @@ static int attn_shape_check(uint32_t cache_type, size_t page_size, size_t kv_hea
     if (act_type != OJAS_B200_F32 && act_type != cache_type) return no(OJAS_B200_E_UNSUPPORTED, "activations must be f32 or the cache's type");
     if (page_size == 0 || page_size % 16) return no(OJAS_B200_E_UNSUPPORTED, "the page size must be a multiple of 16 tokens");
     if (kv_heads == 0 || kv_heads > 65535 || q_heads == 0 || q_heads > 65536 || q_heads % kv_heads) return no(OJAS_B200_E_ARG, "query heads must be a multiple of the cache's heads");
-    if (M > 0x3fffffffull || max_rows > 0x3fffffffull || max_len > 0x7fffff00ull || M * (q_heads / kv_heads) > 0x3fffffffull)
+    if (M > 0x3fffffffull || max_rows > 0x3fffffffull || max_len > (size_t)ATTN_MOST_KEYS || M * (q_heads / kv_heads) > 0x3fffffffull)
         return no(OJAS_B200_E_LIMIT, "too many rows or keys");
     return 0;
 }

@@ -21,6 +21,9 @@ struct AttnArgs {
     float scale_log2;                    // softmax scale * log2(e)
 };
 
+// Keys are counted in 32 bits, and what rounds their number up to a block, or steps past the last, must not pass them.
+constexpr long long ATTN_MOST_KEYS = 0x7fffff00;
+
 // A row is one (token, query head) pair; the rows of a sequence that share a key head are numbered token * group + head in
 // group, and a tile is `rows` of them.
 struct RowTile {
@@ -97,7 +100,7 @@ __device__ __forceinline__ bool find_tile(const AttnArgs &a, int tile, int rows,
     t.n_rows = n * a.group;
     t.row0 = (int)(tile - before) * rows;
     const int len = __ldg(b.len + t.seq);
-    const long long room = (long long)b.table_stride * b.page_size;
+    const long long room = min((long long)b.table_stride * b.page_size, ATTN_MOST_KEYS);
     t.pos0 = (int)max(-0x40000000ll, min(0x7fffffffll, (long long)len - end + first));   // where the append puts the row, whatever lies outside the call
     t.len = (int)max(0ll, min((long long)len, room));
     if (lane == 0 && n > 0 && ((long long)len > room || len < n || n > b.max_rows)) atomicOr(b.status, OJAS_ST_BATCH);

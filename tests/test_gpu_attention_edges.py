@@ -332,3 +332,20 @@ def test_scales_of_any_sign(gpu, act, cache, dim, rows, scale):
     gpu.sync()
     want, weight, vmax = b.attention_exact(q, 8, scale=scale)
     check(out, want, attention_bound(want, weight, vmax, dim, max(b.lens), act, cache, 2 if act == F32 else 1))
+
+
+@pytest.mark.parametrize("rows,act", [(1, F32), (100, F16)])
+def test_a_length_of_31_bits_is_reported(gpu, rows, act):
+    """Longer than max_len may be, with a table that would hold it: no key of it is read, the rows give zeros."""
+    b = Batch([rows], [rows], kv_heads=1, dim=64, page=16, seed=3)
+    b.lens, b.stride, b.table = [2**31 - 1], 2**27, torch.full((1, 2**27), -1, dtype=torch.int32)
+    b.upload(gpu)
+    q = randn(1, rows, 4, 64, dtype=TORCH[act]).cuda()
+    out = torch.full_like(q, 77.0)
+    torch.cuda.synchronize()
+    gpu.attention(b.kv, b.seqs, buf(q), buf(out), rows, 4, act_type=act, window=16)
+    with pytest.raises(ob.OjasB200Error) as e:
+        gpu.sync()
+    assert e.value.code == -5 and "batch" in str(e.value)
+    torch.cuda.synchronize()
+    assert (out == 0).all()
