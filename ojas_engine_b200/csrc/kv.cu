@@ -256,7 +256,7 @@ extern "C" int ojas_b200_kv_append(ojas_b200_ctx *ctx, const ojas_b200_kv *kv, c
     a.batch = {seqs->cu, seqs->len, seqs->table, (int)seqs->n_seqs, (int)seqs->table_stride, (long long)M, (int)kv->pages, (int)kv->page_size, (int)seqs->max_rows, ctx->dev_status};
     a.x_type = x_type; a.q_type = q_type; a.c_type = kv->type;
     a.q_heads = (int)q_heads; a.kv_heads = (int)kv->heads; a.dim = (int)kv->dim;
-    const bool vec = rope_vec_ok(a.rot, a.dim, a.interleaved) && rope_rows_aligned(k, x_type, a.k_stride) && rope_rows_aligned(v, x_type, a.v_stride) &&
+    const bool vec = rope_vec_ok(a.rot, a.dim) && rope_rows_aligned(k, x_type, a.k_stride) && rope_rows_aligned(v, x_type, a.v_stride) &&
                      (q_heads == 0 || (rope_rows_aligned(q, x_type, a.q_stride) && rope_rows_aligned(q_out, q_type, a.q_out_stride)));
     const size_t smem = (size_t)((a.rot / 2 + 1) / 2) * sizeof(float4);
     DeviceGuard guard(ctx->device);

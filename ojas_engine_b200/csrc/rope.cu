@@ -97,7 +97,6 @@ struct RopeArgs {
     const uint64_t *turns;
     float magnitude;
     long long x_stride, y_stride;      // elements between tokens
-    long long M;
     uint32_t x_type, y_type;
     int heads, dim, rot;
     bool interleaved;
@@ -141,9 +140,9 @@ extern "C" int ojas_b200_rope_rows(ojas_b200_ctx *ctx, const ojas_b200_rope *rop
     a.x = x; a.y = y; a.pos = pos; a.turns = rope->turns; a.magnitude = rope->magnitude;
     a.x_stride = (long long)(x_stride ? x_stride : heads * dim);
     a.y_stride = (long long)(y_stride ? y_stride : heads * dim);
-    a.M = (long long)M; a.x_type = x_type; a.y_type = y_type;
+    a.x_type = x_type; a.y_type = y_type;
     a.heads = (int)heads; a.dim = (int)dim; a.rot = (int)rope->rot_dim; a.interleaved = layout == OJAS_B200_ROPE_INTERLEAVED;
-    const bool vec = rope_vec_ok(a.rot, a.dim, a.interleaved) && rope_rows_aligned(x, x_type, a.x_stride) && rope_rows_aligned(y, y_type, a.y_stride);
+    const bool vec = rope_vec_ok(a.rot, a.dim) && rope_rows_aligned(x, x_type, a.x_stride) && rope_rows_aligned(y, y_type, a.y_stride);
     const int units = rope_units(vec ? 4 : 1, a.rot, a.dim);
     const dim3 block(units < 256 ? units : 256, units < 256 ? 256 / units : 1);
     const size_t smem = (size_t)((a.rot / 2 + 1) / 2) * sizeof(float4);

@@ -19,7 +19,7 @@ __device__ __forceinline__ float2 rope_angle(int pos, uint64_t turns, float magn
 // Units a head is cut into: VEC pairs each, then 2 VEC passing elements each.
 __host__ __device__ inline int rope_units(int vec, int rot, int dim) { return rot / 2 / vec + (dim - rot + 2 * vec - 1) / (2 * vec); }
 // Four pairs at a time need whole vectors in both halves of the rotated part and behind it.
-static inline bool rope_vec_ok(int rot, int dim, bool) { return rot % 8 == 0 && (dim - rot) % 8 == 0; }
+static inline bool rope_vec_ok(int rot, int dim) { return rot % 8 == 0 && (dim - rot) % 8 == 0; }
 static inline bool rope_rows_aligned(const void *p, uint32_t type, long long stride) {
     return (uintptr_t)p % (4 * elem_bytes(type)) == 0 && stride % 4 == 0;
 }
