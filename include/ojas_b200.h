@@ -285,6 +285,9 @@ enum { OJAS_B200_ROPE_HALF = 0, OJAS_B200_ROPE_INTERLEAVED = 1 };
  *   orig_len  > 0: by parts.  A pair that turns r_i = orig_len * f_i / 2 pi times within the original context keeps its
  *                  frequency for r_i >= beta_fast, has it divided by factor for r_i <= beta_slow, and is mixed linearly in
  *                  r_i between.
+ * A mix that is linear in the pair's index between the two bounds, which takes parameters of the same names, gives other
+ * frequencies (less than half in places): where a model was trained with that one, pass its frequencies as freq_factors with
+ * orig_len 0 and factor 1, freq_factors[i] = 1 / (keep_i + (1 - keep_i) / factor).
  * Rotated values are multiplied by magnitude.  create allocates rot_dim / 2 words on the device and copies them there (it
  * waits for the copy: set-up only); destroy frees them (after the launches that use them have ended).  A rotation serves
  * every context of its device and may outlive the one it was made with. */
@@ -357,8 +360,10 @@ OJAS_B200_API int ojas_b200_kv_append_check(size_t kv_heads, size_t dim, size_t 
  * up to its own position (causal != 0), or all of them; with window > 0 (causal only) at most the last `window`, its own
  * included.  q head h reads cache head h / (q_heads / heads).  A row that sees nothing gives zeros.  q and out have type
  * act_type: f32, or the cache's type; scale * log2(e) is finite in f32; they start on 16 bytes, strides are multiples of 4 elements, and they must not overlap.
- * f32 activations keep 22 bits through both products over an f16 cache, 16 over a bf16 cache; 16-bit ones are rounded where
- * the probabilities enter the second product and at the end.  Sums and softmax statistics are f32.
+ * f32 activations keep 22 bits through both products over an f16 cache, 16 over a bf16 cache; with 16-bit ones the
+ * probabilities are rounded to that type once where they enter the second product, except in calls of at most eight rows per
+ * cache head (max_rows * q_heads / heads), where they keep two terms too, and the result at the end.  Sums and softmax
+ * statistics are f32.
  * Behind a sequence's end the cache may hold anything; a key that only some rows of a call see must be finite for the
  * others.  workspace: caller-owned scratch of ojas_b200_attention_workspace_bytes (0: may be null), 256-byte aligned, not
  * shared by calls that may run at the same time. */

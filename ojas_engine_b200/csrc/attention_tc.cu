@@ -17,7 +17,9 @@
 //
 // f32 activations enter as two 16-bit terms (TERMS = 2): Q = Qhi + Qlo against the same K, P = Phi + Plo against the same V, twice the
 // MMAs; rows of q are scaled by a power of two so that both terms are in f16's range.  16-bit activations are exact as they
-// are and P is rounded once (relative 2^-12 for f16, 2^-9 for bf16, random over the keys).
+// are and P is rounded once (by 2^-11 at most for f16, 2^-8 for bf16, random over the keys): results of unit-normal values are off by
+// 2.6e-4 and 2.3e-3 of their norm, 2.0e-4 and 1.7e-3 of it the rounding of the result itself.  Two terms of P for them too would
+// take an 8192-token f16 prompt from 613 to 801 us, a window of 1024 over heads of 64 from 111 to 125, 35 drafted rows from 25.4 to 27.1.
 //
 // The tensor cores cut what they add to an accumulator: every instruction takes up to 2^-23 off |O|, always towards zero, and
 // thousands of them over a long context took 1.2e-5 off an f32 result (12 000 keys).  With f32 activations O is therefore added,

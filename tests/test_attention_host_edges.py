@@ -135,3 +135,16 @@ def test_a_scale_stays_finite_in_powers_of_two(scale, ok):
     seqs = runtime._lib.SeqsStruct(256, 512, 1024, 3, 8, 4, 100)
     rc = runtime._lib.load().ojas_b200_attention_check(ob.F16, 16, 2, 128, ob.F32, 8, 1024, 0, 4096, 0, scale, 1, 0, C.byref(seqs), 12, None, 0)
     assert rc == (0 if ok else -1)
+
+
+def test_a_mix_over_the_index_goes_in_as_factors():
+    """The other scaling by parts, linear in the pair's index between the indices where a pair turns beta_fast and beta_slow times:
+    given as factors, which are f32 (half a step, 2^-24 relative at most)."""
+    rot, base, orig, factor, fast, slow = 128, 10000.0, 4096, 8.0, 32.0, 1.0
+    f = base ** (-2 * np.arange(rot // 2) / rot)
+    index = [rot * np.log(orig / (2 * np.pi * turns)) / (2 * np.log(base)) for turns in (fast, slow)]
+    keep = 1 - np.clip((np.arange(rot // 2) - np.floor(index[0])) / (np.ceil(index[1]) - np.floor(index[0])), 0, 1)
+    want = f * keep + f / factor * (1 - keep)
+    assert np.allclose(ob.rope_frequencies(rot, base, freq_factors=1 / (keep + (1 - keep) / factor)), want, rtol=2.0**-24, atol=0)
+    turns = ob.rope_frequencies(rot, base, factor=factor, orig_len=orig, beta_fast=fast, beta_slow=slow)
+    assert 0.4 < (turns / want).min() < 0.5                     # the two forms are not the same
