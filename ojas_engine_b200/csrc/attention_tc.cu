@@ -56,6 +56,7 @@ struct AtShape {
     static constexpr int COL_SUM = 384;
     static constexpr int CHUNK = Q_BYTES / (SOFT_WARPS * 32) < 256 ? Q_BYTES / (SOFT_WARPS * 32) : 256;   // bytes of a row that the epilogue stages at a time
     static_assert(SOFT_WARPS * 32 * CHUNK <= Q_BYTES, "the epilogue stages rows where Q was");
+    static_assert(CHUNK >= 64 && OUT % 32 == 0, "a chunk is 16 or whole 32s of f32 columns, whole 32s of 16-bit ones");
     static_assert(STAGES >= 3, "a K and a V block in use and one on the way");
 };
 
@@ -509,7 +510,7 @@ __global__ void __launch_bounds__(AtShape<D, TERMS, TILES>::THREADS, 1) attn_til
 #pragma unroll 1
                 for (int c0 = 0; c0 < S::OUT; c0 += per) {
 #pragma unroll 1
-                    for (int c = c0; c < c0 + per; c += 32) {
+                    for (int c = c0 & ~31; c < c0 + per; c += 32) {                    // (16 f32 columns: the half of 32 that the chunk holds)
                         float o[32];
                         if (blocks > 0) {
                             at_ld32(o_col + c, o);
@@ -534,7 +535,8 @@ __global__ void __launch_bounds__(AtShape<D, TERMS, TILES>::THREADS, 1) attn_til
                         if (es == 4) {
 #pragma unroll
                             for (int i = 0; i < 8; i++)
-                                *reinterpret_cast<float4 *>(row_at + (((p0 + i) ^ (lane & TURN)) << 4)) = make_float4(o[4 * i] * by, o[4 * i + 1] * by, o[4 * i + 2] * by, o[4 * i + 3] * by);
+                                if (S::CHUNK >= 128 || (unsigned)(p0 + i) < (unsigned)PIECES)
+                                    *reinterpret_cast<float4 *>(row_at + (((p0 + i) ^ (lane & TURN)) << 4)) = make_float4(o[4 * i] * by, o[4 * i + 1] * by, o[4 * i + 2] * by, o[4 * i + 3] * by);
                         } else {
 #pragma unroll
                             for (int i = 0; i < 4; i++)

@@ -349,3 +349,16 @@ def test_a_length_of_31_bits_is_reported(gpu, rows, act):
     assert e.value.code == -5 and "batch" in str(e.value)
     torch.cuda.synchronize()
     assert (out == 0).all()
+
+
+@pytest.mark.parametrize("act,cache", [(F32, F16), (F32, BF16), (F16, F16), (BF16, BF16)])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("rows,lens,heads,group", [([2], [2534], 3, 17), ([8, 8], [1355, 410], 2, 9), ([20, 1], [3000, 100], 1, 5), ([120], [5000], 1, 1), ([130, 30], [4000, 3999], 1, 2)])
+def test_one_tile_split_along_the_keys(gpu, act, cache, dim, rows, lens, heads, group):
+    """Between what the kernel for few rows takes and two tiles of 128 rows, with the keys split: unnormalized f32 sums leave the
+    kernel whatever the activations are."""
+    b = Batch(rows, lens, kv_heads=heads, dim=dim, page=192 if len(rows) == 1 else 32, nhd=len(rows) == 1, cache=cache, seed=dim).upload(gpu)
+    assert splits(gpu, b, heads * group, act) > 1
+    q = randn(1, b.M, heads * group, dim).to(TORCH[act])
+    want, weight, vmax = b.attention_exact(q, heads * group)
+    check(attend(gpu, b, q, heads * group, act), want, attention_bound(want, weight, vmax, dim, max(lens), act, cache, 2 if act == F32 else 1))
